@@ -1243,6 +1243,68 @@ typedef struct {
 } mdp_raycaster_camera_args_t;
 int mdp_raycaster_camera_update(int num_envs, const mdp_raycaster_camera_args_t* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Policy side: categorical actions and gradient clipping (isaaclab_amd/rl)
+ * ------------------------------------------------------------------------------------------
+ * The rows of `logits` (rows, vocab; row stride ld, unit stride inside a row; element type MDP_DTYPE_*) are unnormalised
+ * log-probabilities.  Allowed entries of a row: mask != 0 (NULL = all) and logit > -inf. */
+enum { MDP_DTYPE_F32 = 0, MDP_DTYPE_BF16 = 1, MDP_DTYPE_F16 = 2, MDP_DTYPE_NUM = 3 };
+
+/* One entry of every row from one uniform u in [0, 1) each -- injected like the draws of mdp_sample (LAB/utils/math.py:
+ * 1233-1421), or NULL: the generator `state` = device {seed, epoch}, whose epoch the call advances in stream order.
+ *   weights  w_i = exp((x_i - max) / temperature); temperature 0: the largest logit, lowest index first
+ *   kept     the first top_k entries in the order (logit falling, index rising) (<= 0: all), of these the shortest prefix that
+ *            holds a share top_p of their mass (>= 1: all; one entry at least), of these the ones with w_i >= min_p
+ *   answer   the first kept i in index order with (kept mass up to and with i) > u * (kept mass); log_prob = ln of its share
+ * All sums in 64 bits.  Settings are scalars, or per-row device arrays where the pointer is not NULL.  A row without allowed
+ * entries gives action -1, log_prob 0; one that holds a NaN or +inf among its allowed entries, or a temperature that is
+ * negative or NaN, gives action -1, log_prob NaN. */
+typedef struct {
+    const void* logits; int64_t ld; int64_t rows; int64_t vocab; int32_t dtype; int32_t pad0;
+    const uint8_t* mask; int64_t ld_mask;
+    const float* temperature; const int32_t* top_k; const float* top_p; const float* min_p;
+    float temperature_scalar; int32_t top_k_scalar; float top_p_scalar; float min_p_scalar;
+    const float* u;
+    uint64_t* state;
+    int64_t* actions;                  /* (rows) out */
+    float* log_prob;                   /* (rows) out */
+} mdp_categorical_sample_t;
+int mdp_categorical_sample(const mdp_categorical_sample_t* args, void* stream);
+
+/* Log-probability of actions[row] and entropy of softmax(logits / temperature) over the allowed entries of every row.
+ * Action -1 (a row that had nothing to choose from): log_prob 0; an action that is not allowed: -inf; one outside
+ * [-1, vocab): NaN.  A row without allowed entries has entropy 0.  stats (rows, 3), or NULL: what _grad reads.
+ * _grad: grad_logits = gradient of sum(grad_log_prob * log_prob + grad_entropy * entropy) by the logits, in their type
+ * (either may be NULL: zeros); entries that are not allowed get 0.  Settings, mask and actions as in the forward call. */
+typedef struct {
+    const void* logits; int64_t ld; int64_t rows; int64_t vocab; int32_t dtype; float temperature_scalar;
+    const uint8_t* mask; int64_t ld_mask;
+    const int64_t* actions;
+    const float* temperature;          /* (rows) or NULL: temperature_scalar */
+    float* log_prob;                   /* (rows) out */
+    float* entropy;                    /* (rows) out */
+    float* stats;
+} mdp_categorical_eval_t;
+int mdp_categorical_evaluate(const mdp_categorical_eval_t* args, void* stream);
+int mdp_categorical_evaluate_grad(const mdp_categorical_eval_t* args, const float* grad_log_prob, const float* grad_entropy,
+                                  void* grad_logits, int64_t ld_grad, void* stream);
+
+/* The norm of many gradients taken as one vector, and clipping to it.  `grads` is a HOST array (read during the call) of dense
+ * device tensors.  norm_kind: 2 = root of the sum of squares, 1 = sum of magnitudes, 0 = largest magnitude (inf norm); sums
+ * and squares in 64 bits, in an order that depends on the sizes alone.
+ * mdp_grad_norm:  *norm (device float).
+ * mdp_grad_clip:  the same, then out = grad * min(1, max_norm / (norm + 1e-6)) for every tensor; out may be grad itself (left
+ * untouched where nothing is clipped) or another tensor of the same type or float32.  A norm that is infinite makes the factor
+ * 0, one that is NaN makes it NaN.  Outputs overlap neither each other nor another tensor's gradient (MDP_ERR_INVALID).
+ * workspace: mdp_grad_workspace(n) doubles, not shared by calls that may run at the same time; NULL is refused. */
+typedef struct {
+    const void* grad; void* out; int64_t count; int32_t dtype; int32_t out_dtype;
+} mdp_grad_t;
+int64_t mdp_grad_workspace(int64_t num_grads);
+int mdp_grad_norm(const mdp_grad_t* grads, int64_t num_grads, int norm_kind, double* workspace, float* norm, void* stream);
+int mdp_grad_clip(const mdp_grad_t* grads, int64_t num_grads, int norm_kind, double max_norm, double* workspace, float* norm,
+                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,7 @@ import fails loudly, and every wrapper raises if a tensor does not live on a HIP
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import re
@@ -336,6 +337,33 @@ class MdpSceneUpdate(C.Structure):
     ]
 
 
+class MdpCategoricalSample(C.Structure):
+    """Mirror of ``mdp_categorical_sample_t``."""
+
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("rows", C.c_int64), ("vocab", C.c_int64), ("dtype", C.c_int32),
+                ("pad0", C.c_int32), ("mask", C.c_void_p), ("ld_mask", C.c_int64),
+                ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("temperature_scalar", C.c_float), ("top_k_scalar", C.c_int32), ("top_p_scalar", C.c_float),
+                ("min_p_scalar", C.c_float),
+                ("u", C.c_void_p), ("state", C.c_void_p), ("actions", C.c_void_p), ("log_prob", C.c_void_p)]
+
+
+class MdpCategoricalEval(C.Structure):
+    """Mirror of ``mdp_categorical_eval_t``."""
+
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("rows", C.c_int64), ("vocab", C.c_int64), ("dtype", C.c_int32),
+                ("temperature_scalar", C.c_float), ("mask", C.c_void_p), ("ld_mask", C.c_int64),
+                ("actions", C.c_void_p), ("temperature", C.c_void_p), ("log_prob", C.c_void_p), ("entropy", C.c_void_p),
+                ("stats", C.c_void_p)]
+
+
+class MdpGrad(C.Structure):
+    """Mirror of ``mdp_grad_t``."""
+
+    _fields_ = [("grad", C.c_void_p), ("out", C.c_void_p), ("count", C.c_int64), ("dtype", C.c_int32),
+                ("out_dtype", C.c_int32)]
+
+
 def _parse_defines(path: str, prefix: str) -> dict[str, int]:
     out = {}
     with open(path) as f:
@@ -360,6 +388,7 @@ def _parse_enum(path: str, prefix: str) -> dict[str, int]:
 _HDR = os.path.join(os.path.dirname(_HERE), "include", "mdp_hip.h")
 MATH_OPS = _parse_enum(_HDR, "MDP_MATH_")
 ACT_KINDS = _parse_enum(_HDR, "MDP_ACT_")
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # MDP_DTYPE_*
 PROG_OBS, PROG_REWARD, PROG_TERMINATION = 0, 1, 2
 with open(_HDR) as _f:
     MDP_STATS_MAX_SOURCES = int(re.search(r"#define\s+MDP_STATS_MAX_SOURCES\s+(\d+)", _f.read()).group(1))
@@ -463,6 +492,14 @@ def rows(t: torch.Tensor, name: str = "tensor") -> tuple[torch.Tensor, int]:
 
 def stream(device=None):
     return torch.cuda.current_stream(device).cuda_stream
+
+
+byref = C.byref
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one: a launch on its stream needs that."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def device_index(device) -> int:

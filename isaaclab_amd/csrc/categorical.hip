@@ -11,6 +11,8 @@
 #include "mdp_device.hpp"
 #include "mdp_host.hpp"
 #include "elements_device.hpp"
+#include <algorithm>
+#include <type_traits>
 
 using namespace mdp;
 
@@ -261,7 +263,99 @@ __global__ __launch_bounds__(THREADS) void k_sample_row(SampleArgs g) {
 
 __global__ void k_state_advance(unsigned long long* state) { state[1] += 1ull; }
 
+// -- rows ---------------------------------------------------------------------------------------------------------------
+// A row as the 16-byte chunks of memory that it touches: chunk j holds entries j N - shift .. j N - shift + N - 1, of which
+// the first and the last chunk may hold some that are not the row's.  Those are never read: an edge chunk is read entry by
+// entry.  A masked entry reads as -inf.
+template <typename T>
+struct Row {
+    static constexpr int N = Chunk<T>::N;
+    const T* x;
+    const uint8_t* mask;
+    int V, shift;
+    bool mask_chunks;                                  // the mask's chunks start on N-byte boundaries where the logits' do
+
+    MDP_DEV Row(const void* logits, int64_t ld, const uint8_t* m, int64_t ld_mask, int vocab, int64_t row)
+        : x((const T*)logits + row * ld), mask(m ? m + row * ld_mask : nullptr), V(vocab),
+          shift((int)(((uintptr_t)x & 15) / sizeof(T))), mask_chunks((((uintptr_t)mask - (uintptr_t)shift) & (N - 1)) == 0) {}
+    MDP_DEV int chunks() const { return (V + shift + N - 1) / N; }
+    MDP_DEV int full_first() const { return shift ? 1 : 0; }
+    MDP_DEV int full_end() const { return (V + shift) / N; }     // one past the last full chunk
+    MDP_DEV bool full(int j) const { return j >= full_first() && j < full_end(); }
+    MDP_DEV Chunk<T> chunk(int j) const { return Chunk<T>{*(const uint4*)(x + (j * N - shift))}; }
+    MDP_DEV bool allowed(int i) const { return !mask || mask[i]; }
+    MDP_DEV float entry(int i) const { return allowed(i) ? to_f32(x[i]) : -kInf; }
+    // the mask of a full chunk, one bit an entry
+    MDP_DEV uint32_t allowed_chunk(int j) const {
+        const uint8_t* m = mask + (j * N - shift);
+        uint32_t bits = 0;
+        if (mask_chunks) {
+            uint32_t w[2];
+            if constexpr (N == 4) { w[0] = *(const uint32_t*)m; w[1] = 0; }
+            else { const uint2 q = *(const uint2*)m; w[0] = q.x; w[1] = q.y; }
+#pragma unroll
+            for (int e = 0; e < N; ++e) bits |= ((w[e / 4] >> (8 * (e % 4))) & 0xffu ? 1u : 0u) << e;
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) bits |= (m[e] ? 1u : 0u) << e;
+        }
+        return bits;
+    }
+    // entries of chunk j; what is not the row's, or masked, is -inf
+    template <bool MASK>
+    MDP_DEV void load(int j, float (&v)[N]) const {
+        if (full(j)) {
+            const Chunk<T> c = chunk(j);
+            const uint32_t ok = MASK ? allowed_chunk(j) : ~0u;
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = ok >> e & 1u ? c.at(e) : -kInf;
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int i = j * N - shift + e;
+                v[e] = i >= 0 && i < V && (!MASK || mask[i]) ? to_f32(x[i]) : -kInf;
+            }
+        }
+    }
+};
+
+// the larger of two numbers, b where a is a NaN (one instruction, without fmaxf's canonicalisation of its operands)
+MDP_DEV float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, kInf); }
+
+// lane i gets lane i ^ m's value (m < 4), or, for m = 4 and 8, that of the lane mirrored inside 8 or 16: what a reduction
+// needs whose groups of m already agree
+template <int M>
+MDP_DEV float across(float v) {
+    const int x = __float_as_int(v);
+    if constexpr (M == 1) return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0xB1, 0xf, 0xf, true));        // quad_perm 1 0 3 2
+    else if constexpr (M == 2) return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0x4E, 0xf, 0xf, true));   // quad_perm 2 3 0 1
+    else if constexpr (M == 4) return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, true));  // row_half_mirror
+    else if constexpr (M == 8) return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, true));  // row_mirror
+    else return __shfl_xor(v, M);
+}
+template <int G, class F>
+MDP_DEV float over_group(float v, F&& f) {             // every lane of a group of G gets the result
+    if constexpr (G > 1) v = f(v, across<1>(v));
+    if constexpr (G > 2) v = f(v, across<2>(v));
+    if constexpr (G > 4) v = f(v, across<4>(v));
+    if constexpr (G > 8) v = f(v, across<8>(v));
+    if constexpr (G > 16) v = f(v, across<16>(v));
+    if constexpr (G > 32) v = f(v, across<32>(v));
+    return v;
+}
+template <int G>
+MDP_DEV float group_max(float v) { return over_group<G>(v, [](float a, float b) { return larger(a, b); }); }
+template <int G>
+MDP_DEV float group_sum(float v) { return over_group<G>(v, [](float a, float b) { return a + b; }); }
+
 // -- evaluation -------------------------------------------------------------------------------------------------------
+// One pass: about the largest entry m so far, s = sum w and t = sum w log2 w with w = 2^((x - m) log2(e) / T).  Entries that
+// are not allowed read as -inf and add nothing; a NaN or +inf makes s a NaN.
+//
+// Bound by memory: a bfloat16 entry costs about ten issue slots (four of them v_exp_f32), two thirds of what a CU issues in
+// the time its share of the memory rate brings one.
+constexpr float kLog2E = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
 struct EvalArgs {
     const void* logits; int64_t ld;
     const uint8_t* mask; int64_t ld_mask;
@@ -281,104 +375,223 @@ struct GradArgs {
     const float* stats;
     const float* grad_log_prob; const float* grad_entropy;
     void* grad; int64_t ld_grad;
+    int pieces;                                        // blocks a row
 };
 
-// ln w, held at or above -200 (where w is 0 in 32 bits) so that 0 * ln 0 is 0; a NaN stays one
-MDP_DEV float log_weight(float x, float m, float inv_t) {
-    const float d = (x - m) * inv_t;
-    return d < -200.0f ? -200.0f : d;
+MDP_DEV float inverse_temperature(const float* per_row, float scalar, int64_t row) {
+    const float t = per_row ? per_row[row] : scalar;
+    return t > 0.0f && t < kInf ? 1.0f / t : __builtin_nanf("");
 }
 
-// running (m, s, t) of a softmax: s = sum w, t = sum w ln w about the largest entry so far
 struct Running {
     float m, s, t;
     MDP_DEV static Running none() { return Running{-__FLT_MAX__, 0.0f, 0.0f}; }
-    MDP_DEV void move(float to, float inv_t) {        // about another maximum >= m
-        const float d = log_weight(m, to, inv_t), f = expf(d);
+    MDP_DEV void move(float to, float c) {             // about another maximum >= m
+        float d = (m - to) * c;
+        d = d < -300.0f ? -300.0f : d;                 // 2^-300 is 0: 0 * inf must not arise
+        const float f = __builtin_amdgcn_exp2f(d);
         t = f * (t + d * s);
         s *= f;
         m = to;
     }
-    MDP_DEV void add(float x, float inv_t) {
-        if (x > m) move(x, inv_t);
-        const float d = log_weight(x, m, inv_t), e = expf(d);
-        s += e;
-        t += e * d;
-    }
-    MDP_DEV void join(Running o, float inv_t) {
-        const float to = fmaxf(m, o.m);
-        move(to, inv_t);
-        o.move(to, inv_t);
-        s += o.s;
-        t += o.t;
+    // n entries, none above m; summed on their own first: short chains of additions
+    template <int N>
+    MDP_DEV void add(const float (&v)[N], float c) {
+        float cs = 0.0f, ct = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float d = (v[e] - m) * c, w = __builtin_amdgcn_exp2f(d);
+            cs += w;
+            ct = fmaf(w, larger(d, -300.0f), ct);      // w is 0 there, and a NaN shows in s
+        }
+        s += cs;
+        t += ct;
     }
 };
 
-template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_evaluate_row(EvalArgs g) {
-    __shared__ Running part[THREADS / 64];
-    const int64_t row = blockIdx.x;
-    const int V = g.vocab, tid = threadIdx.x;
-    const T* x = (const T*)g.logits + row * g.ld;
-    const uint8_t* mask = g.mask ? g.mask + row * g.ld_mask : nullptr;
-    const float temp = g.temperature ? g.temperature[row] : g.temperature_s;
-    const float inv_t = temp > 0.0f ? 1.0f / temp : __builtin_nanf("");
-    Running r = Running::none();
-    for (int i = tid; i < V; i += THREADS)
-        if (!mask || mask[i]) r.add(to_f32(x[i]), inv_t);
-    for (int o = 32; o > 0; o >>= 1) {
-        Running q;
-        q.m = __shfl_xor(r.m, o); q.s = __shfl_xor(r.s, o); q.t = __shfl_xor(r.t, o);
-        r.join(q, inv_t);
-    }
-    if ((tid & 63) == 0) part[tid >> 6] = r;
-    __syncthreads();
-    if (tid) return;
-    for (int w = 1; w < THREADS / 64; ++w) r.join(part[w], inv_t);
-    const float log_s = logf(r.s);
-    const float h = r.s == 0.0f ? 0.0f : log_s - r.t / r.s;
+template <typename T>
+MDP_DEV void finish_row(const EvalArgs& g, const Row<T>& r, int64_t row, float m, float s, float t, float inv_t) {
+    const float log_s = logf(s);
+    const float h = s == 0.0f ? 0.0f : log_s - kLn2 * (t / s);
     const int64_t a = g.actions[row];
     float lp;
     if (a == -1) lp = 0.0f;
-    else if (a < 0 || a >= V) lp = __builtin_nanf("");
-    else if (mask && !mask[a]) lp = r.s == r.s ? -kInf : r.s;
-    else lp = (to_f32(x[a]) - r.m) * inv_t - log_s;
+    else if (a < 0 || a >= r.V) lp = __builtin_nanf("");
+    else if (!r.allowed((int)a)) lp = s == s ? -kInf : s;
+    else lp = (to_f32(r.x[a]) - m) * inv_t - log_s;
     g.log_prob[row] = lp;
     g.entropy[row] = h;
     if (g.stats) {
-        g.stats[3 * row] = r.m;
+        g.stats[3 * row] = m;
         g.stats[3 * row + 1] = log_s;
         g.stats[3 * row + 2] = h;
     }
 }
 
-template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_evaluate_grad(GradArgs g) {
+// Rows of up to G K chunks: G lanes of a wave hold a row in registers, so its maximum is known before the first exponential.
+template <typename T, bool MASK, int G, int K>
+__global__ __launch_bounds__(256) void k_evaluate_short(EvalArgs g) {
+    constexpr int N = Chunk<T>::N;
+    const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int lane = threadIdx.x % G;
+    if (row >= g.rows) return;
+    const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
+    const float inv_t = inverse_temperature(g.temperature, g.temperature_s, row), c = inv_t * kLog2E;
+    float v[K][N];
+#pragma unroll
+    for (int k = 0; k < K; ++k) r.template load<MASK>(k * G + lane, v[k]);
+    Running q = Running::none();
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < N; ++e) q.m = larger(v[k][e], q.m);
+    q.m = group_max<G>(q.m);
+#pragma unroll
+    for (int k = 0; k < K; ++k) q.add(v[k], c);
+    q.s = group_sum<G>(q.s);
+    q.t = group_sum<G>(q.t);
+    if (lane == 0) finish_row(g, r, row, q.m, q.s, q.t, inv_t);
+}
+
+// Longer rows: a block a row, four chunks a thread in flight, their maximum looked at once.
+template <typename T, bool MASK>
+__global__ __launch_bounds__(256) void k_evaluate_long(EvalArgs g) {
+    constexpr int N = Chunk<T>::N, B = 4;
+    __shared__ float wave_m[4], wave_s[4], wave_t[4];
     const int64_t row = blockIdx.x;
-    const int V = g.vocab;
-    const T* x = (const T*)g.logits + row * g.ld;
-    T* out = (T*)g.grad + row * g.ld_grad;
-    const uint8_t* mask = g.mask ? g.mask + row * g.ld_mask : nullptr;
-    const float temp = g.temperature ? g.temperature[row] : g.temperature_s;
-    const float inv_t = temp > 0.0f ? 1.0f / temp : __builtin_nanf("");
-    const float m = g.stats[3 * row], log_s = g.stats[3 * row + 1], h = g.stats[3 * row + 2];
-    const int64_t a = g.actions[row];
-    float gl = g.grad_log_prob ? g.grad_log_prob[row] : 0.0f;
-    const float ge = g.grad_entropy ? g.grad_entropy[row] : 0.0f;
-    if (a == -1) gl = 0.0f;
-    else if (a < 0 || a >= V) gl = __builtin_nanf("");
-    const bool empty = log_s == -kInf;
-    for (int i = threadIdx.x; i < V; i += THREADS) {
-        float y = 0.0f;
-        const float v = to_f32(x[i]);
-        if (!(mask && !mask[i]) && v != -kInf && !empty) {
-            const float lw = log_weight(v, m, inv_t), lp = lw - log_s, p = expf(lp);
-            y = -p * (gl + ge * (lp + h));
-            if (i == a) y += gl;
-            y *= inv_t;
+    const int tid = threadIdx.x;
+    const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
+    const float inv_t = inverse_temperature(g.temperature, g.temperature_s, row), c = inv_t * kLog2E;
+    const int first = r.full_first(), end = r.full_end();
+    Running q = Running::none();
+    for (int j0 = first + tid; j0 < end; j0 += 256 * B) {
+        Chunk<T> raw[B];
+        uint32_t ok[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int j = j0 + 256 * b;
+            ok[b] = 0;
+            if (j < end) {
+                raw[b] = r.chunk(j);
+                ok[b] = MASK ? r.allowed_chunk(j) : ~0u;
+            }
         }
-        from_f32(y, out[i]);
+        float v[B][N], top = q.m;
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                v[b][e] = ok[b] >> e & 1u ? raw[b].at(e) : -kInf;
+                top = larger(v[b][e], top);
+            }
+        if (top > q.m) q.move(top, c);
+#pragma unroll
+        for (int b = 0; b < B; ++b) q.add(v[b], c);
     }
+    // the entries of the two edge chunks, one a lane
+    const int head = first ? min(r.V, N - r.shift) : 0, tail = max(head, end * N - r.shift);
+    const int i = tid < head ? tid : tail + tid - head;
+    if (i < r.V) {
+        const float v[1] = {r.entry(i)};
+        if (v[0] > q.m) q.move(v[0], c);
+        q.add(v, c);
+    }
+    const float wm = group_max<64>(q.m);
+    if ((tid & 63) == 0) wave_m[tid >> 6] = wm;
+    __syncthreads();
+    q.move(larger(larger(wave_m[0], wave_m[1]), larger(wave_m[2], wave_m[3])), c);
+    q.s = group_sum<64>(q.s);
+    q.t = group_sum<64>(q.t);
+    if ((tid & 63) == 0) { wave_s[tid >> 6] = q.s; wave_t[tid >> 6] = q.t; }
+    __syncthreads();
+    if (tid == 0)
+        finish_row(g, r, row, q.m, wave_s[0] + wave_s[1] + wave_s[2] + wave_s[3], wave_t[0] + wave_t[1] + wave_t[2] + wave_t[3], inv_t);
+}
+
+// Gradient of an entry: -p (gl + ge (ln p + H)) / T, and + gl / T at the action, with log2 p = (x - m) log2(e) / T - log2 s.
+template <typename T>
+struct RowGrad {
+    float m, c, log2_s, a0, a1, hot;
+    int action;                                        // -1: none in the row
+    MDP_DEV RowGrad(const GradArgs& g, int64_t row) {
+        const float inv_t = inverse_temperature(g.temperature, g.temperature_s, row);
+        m = g.stats[3 * row];
+        c = inv_t * kLog2E;
+        const float log_s = g.stats[3 * row + 1], h = g.stats[3 * row + 2];
+        log2_s = log_s * kLog2E;
+        const int64_t a = g.actions[row];
+        action = a >= 0 && a < g.vocab ? (int)a : -1;
+        float gl = g.grad_log_prob ? g.grad_log_prob[row] : 0.0f;
+        const float ge = g.grad_entropy ? g.grad_entropy[row] : 0.0f;
+        if (a == -1) gl = 0.0f;
+        else if (action < 0) gl = __builtin_nanf("");
+        hot = gl * inv_t;
+        a0 = -(gl + ge * h) * inv_t;
+        a1 = -ge * kLn2 * inv_t;
+    }
+    MDP_DEV float operator()(float x, int i) const {
+        if (x == -kInf) return 0.0f;
+        const float lp = larger((x - m) * c - log2_s, -300.0f), p = __builtin_amdgcn_exp2f(x != x ? x : lp);
+        float y = p * fmaf(a1, lp, a0);
+        return i == action ? y + hot : y;
+    }
+};
+
+template <typename T, bool MASK, int G, int K>
+__global__ __launch_bounds__(256) void k_grad_short(GradArgs g) {
+    constexpr int N = Chunk<T>::N;
+    const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int lane = threadIdx.x % G;
+    if (row >= g.rows) return;
+    const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
+    T* out = (T*)g.grad + row * g.ld_grad;
+    const bool same = ((uintptr_t)out & 15) == ((uintptr_t)r.x & 15);
+    const RowGrad<T> f(g, row);
+    float v[K][N];
+#pragma unroll
+    for (int k = 0; k < K; ++k) r.template load<MASK>(k * G + lane, v[k]);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int j = k * G + lane, i0 = j * N - r.shift;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[k][e] = f(v[k][e], i0 + e);
+        if (same && r.full(j)) *(uint4*)(out + i0) = Chunk<T>::of(v[k]).raw;
+        else
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (i0 + e >= 0 && i0 + e < r.V) from_f32(v[k][e], out[i0 + e]);
+    }
+}
+
+// Longer rows: `pieces` blocks a row.  Rows are taken from the last one on: those the evaluation read last, so that part of
+// them is still in the caches.
+template <typename T, bool MASK>
+__global__ __launch_bounds__(256) void k_grad_long(GradArgs g) {
+    constexpr int N = Chunk<T>::N;
+    const int64_t row = g.rows - 1 - blockIdx.x / g.pieces;
+    const int piece = blockIdx.x % g.pieces, tid = threadIdx.x;
+    const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
+    T* out = (T*)g.grad + row * g.ld_grad;
+    const bool same = ((uintptr_t)out & 15) == ((uintptr_t)r.x & 15);
+    const RowGrad<T> f(g, row);
+    const int first = r.full_first(), end = r.full_end();
+#pragma unroll 4
+    for (int j = first + piece * 256 + tid; j < end; j += g.pieces * 256) {
+        const Chunk<T> raw = r.chunk(j);
+        const uint32_t ok = MASK ? r.allowed_chunk(j) : ~0u;
+        const int i0 = j * N - r.shift;
+        float v[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = f(ok >> e & 1u ? raw.at(e) : -kInf, i0 + e);
+        if (same) *(uint4*)(out + i0) = Chunk<T>::of(v).raw;
+        else
+#pragma unroll
+            for (int e = 0; e < N; ++e) from_f32(v[e], out[i0 + e]);
+    }
+    if (piece) return;
+    const int head = first ? min(r.V, N - r.shift) : 0, tail = max(head, end * N - r.shift);
+    const int i = tid < head ? tid : tail + tid - head;
+    if (i < r.V) from_f32(f(r.entry(i), i), out[i]);
 }
 
 int check_rows(const char* what, const void* logits, int64_t rows, int64_t vocab, int64_t ld, int dtype, const uint8_t* mask,
@@ -417,6 +630,47 @@ extern "C" int mdp_categorical_sample(const mdp_categorical_sample_t* a, void* s
     return MDP_OK;
 }
 
+namespace {
+
+// The most chunks that a row of `vocab` entries can touch decides how many lanes hold it; beyond 256 chunks (1024 floats, 2048
+// 16-bit entries) a row is a block's.
+template <typename T, bool MASK>
+void launch_evaluate(const EvalArgs& g, hipStream_t s) {
+    const int chunks = (g.vocab + 2 * (Chunk<T>::N - 1)) / Chunk<T>::N;
+#define SHORT(G, K)                                                                                                            \
+    if (chunks <= G * K) {                                                                                                     \
+        hipLaunchKernelGGL((k_evaluate_short<T, MASK, G, K>), dim3((unsigned)((g.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, s, g); \
+        return;                                                                                                                \
+    }
+    SHORT(4, 1) SHORT(4, 2) SHORT(4, 4) SHORT(8, 4) SHORT(16, 4) SHORT(32, 4) SHORT(64, 4)
+#undef SHORT
+    hipLaunchKernelGGL((k_evaluate_long<T, MASK>), dim3((unsigned)g.rows), dim3(256), 0, s, g);
+}
+
+template <typename T, bool MASK>
+void launch_grad(GradArgs g, hipStream_t s) {
+    const int chunks = (g.vocab + 2 * (Chunk<T>::N - 1)) / Chunk<T>::N;
+#define SHORT(G, K)                                                                                                        \
+    if (chunks <= G * K) {                                                                                                 \
+        hipLaunchKernelGGL((k_grad_short<T, MASK, G, K>), dim3((unsigned)((g.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, s, g); \
+        return;                                                                                                            \
+    }
+    SHORT(4, 1) SHORT(4, 2) SHORT(4, 4) SHORT(8, 4) SHORT(16, 4) SHORT(32, 4) SHORT(64, 4)
+#undef SHORT
+    const int64_t most = 0x7fffffff / g.rows;          // a launch's blocks
+    g.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(most, (chunks + 1023) / 1024));
+    hipLaunchKernelGGL((k_grad_long<T, MASK>), dim3((unsigned)(g.rows * g.pieces)), dim3(256), 0, s, g);
+}
+
+template <class F>
+void by_type(int dtype, bool mask, F&& f) {
+    if (dtype == MDP_DTYPE_F32) mask ? f(float{}, std::true_type{}) : f(float{}, std::false_type{});
+    else if (dtype == MDP_DTYPE_BF16) mask ? f(bf16{}, std::true_type{}) : f(bf16{}, std::false_type{});
+    else mask ? f(f16{}, std::true_type{}) : f(f16{}, std::false_type{});
+}
+
+}  // namespace
+
 extern "C" int mdp_categorical_evaluate(const mdp_categorical_eval_t* a, void* stream) {
     MDP_REQUIRE(a, "null arguments");
     if (int rc = check_rows("categorical_evaluate", a->logits, a->rows, a->vocab, a->ld, a->dtype, a->mask, a->ld_mask)) return rc;
@@ -425,12 +679,7 @@ extern "C" int mdp_categorical_evaluate(const mdp_categorical_eval_t* a, void* s
     EvalArgs g{a->logits, a->ld, a->mask, a->ld_mask, (int)a->vocab, a->rows, a->actions, a->temperature, a->temperature_scalar,
                a->log_prob, a->entropy, a->stats};
     hipStream_t s = as_stream(stream);
-    const dim3 grid((unsigned)a->rows);
-    switch (a->dtype) {
-        case MDP_DTYPE_F32: hipLaunchKernelGGL((k_evaluate_row<float, 256>), grid, dim3(256), 0, s, g); break;
-        case MDP_DTYPE_BF16: hipLaunchKernelGGL((k_evaluate_row<bf16, 256>), grid, dim3(256), 0, s, g); break;
-        default: hipLaunchKernelGGL((k_evaluate_row<f16, 256>), grid, dim3(256), 0, s, g); break;
-    }
+    by_type(a->dtype, a->mask, [&](auto t, auto m) { launch_evaluate<decltype(t), decltype(m)::value>(g, s); });
     MDP_LAUNCH_CHECK();
     return MDP_OK;
 }
@@ -443,14 +692,9 @@ extern "C" int mdp_categorical_evaluate_grad(const mdp_categorical_eval_t* a, co
     MDP_REQUIRE(a->actions && a->stats && grad_logits, "categorical_evaluate_grad: null pointer");
     MDP_REQUIRE(ld_grad >= a->vocab, "categorical_evaluate_grad: gradient rows overlap");
     GradArgs g{a->logits, a->ld, a->mask, a->ld_mask, (int)a->vocab, a->rows, a->actions, a->temperature, a->temperature_scalar,
-               a->stats, grad_log_prob, grad_entropy, grad_logits, ld_grad};
+               a->stats, grad_log_prob, grad_entropy, grad_logits, ld_grad, 1};
     hipStream_t s = as_stream(stream);
-    const dim3 grid((unsigned)a->rows);
-    switch (a->dtype) {
-        case MDP_DTYPE_F32: hipLaunchKernelGGL((k_evaluate_grad<float, 256>), grid, dim3(256), 0, s, g); break;
-        case MDP_DTYPE_BF16: hipLaunchKernelGGL((k_evaluate_grad<bf16, 256>), grid, dim3(256), 0, s, g); break;
-        default: hipLaunchKernelGGL((k_evaluate_grad<f16, 256>), grid, dim3(256), 0, s, g); break;
-    }
+    by_type(a->dtype, a->mask, [&](auto t, auto m) { launch_grad<decltype(t), decltype(m)::value>(g, s); });
     MDP_LAUNCH_CHECK();
     return MDP_OK;
 }

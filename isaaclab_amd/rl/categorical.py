@@ -164,7 +164,7 @@ class _Evaluate(torch.autograd.Function):
 
 
 def _temperature(value, logits):
-    if not isinstance(value, torch.Tensor) and not float(value) > 0.0:
+    if not isinstance(value, torch.Tensor) and not float(value) >= 2.0 ** -126:
         raise ValueError(f"temperature must be positive, got {value}")
     return _setting(value, "temperature", torch.float32, logits, 0.0, _MOST)
 
@@ -176,7 +176,8 @@ def evaluate_categorical(logits: torch.Tensor, actions: torch.Tensor, *, tempera
 
     Action -1 (what a row with nothing allowed was given) has log_prob 0 and no gradient through it, an action that is not
     allowed -inf, one outside [-1, vocab) NaN.  A row with nothing allowed has entropy 0 and gradient 0; entries that are not
-    allowed have gradient 0.  A NaN or +inf among the allowed logits makes its row NaN.
+    allowed have gradient 0.  A NaN or +inf among the allowed logits makes its row NaN, and so does a per-row temperature that
+    is not positive and finite.
 
     Inside a captured graph use ``evaluate_categorical_grad``, which does without autograd's own streams and graph nodes."""
     L.require_gpu(logits, "logits")

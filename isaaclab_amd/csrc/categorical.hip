@@ -308,7 +308,7 @@ struct Row {
             const Chunk<T> c = chunk(j);
             const uint32_t ok = MASK ? allowed_chunk(j) : ~0u;
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = ok >> e & 1u ? c.at(e) : -kInf;
+            for (int e = 0; e < N; ++e) v[e] = !MASK || (ok >> e & 1u) ? c.at(e) : -kInf;
         } else {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
@@ -470,10 +470,11 @@ __global__ __launch_bounds__(256) void k_evaluate_long(EvalArgs g) {
 #pragma unroll
         for (int b = 0; b < B; ++b) {
             const int j = j0 + 256 * b;
+            raw[b] = Chunk<T>::lowest();
             ok[b] = 0;
             if (j < end) {
                 raw[b] = r.chunk(j);
-                ok[b] = MASK ? r.allowed_chunk(j) : ~0u;
+                if (MASK) ok[b] = r.allowed_chunk(j);
             }
         }
         float v[B][N], top = q.m;
@@ -481,7 +482,7 @@ __global__ __launch_bounds__(256) void k_evaluate_long(EvalArgs g) {
         for (int b = 0; b < B; ++b)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                v[b][e] = ok[b] >> e & 1u ? raw[b].at(e) : -kInf;
+                v[b][e] = !MASK || (ok[b] >> e & 1u) ? raw[b].at(e) : -kInf;
                 top = larger(v[b][e], top);
             }
         if (top > q.m) q.move(top, c);
@@ -509,16 +510,19 @@ __global__ __launch_bounds__(256) void k_evaluate_long(EvalArgs g) {
 }
 
 // Gradient of an entry: -p (gl + ge (ln p + H)) / T, and + gl / T at the action, with log2 p = (x - m) log2(e) / T - log2 s.
+// Held at or above -300, where p is 0 in 32 bits, an entry that is not allowed gives a zero by itself; only rows that hold a NaN
+// (`whole` false) are told apart entry by entry.
 template <typename T>
 struct RowGrad {
     float m, c, log2_s, a0, a1, hot;
     int action;                                        // -1: none in the row
+    bool whole;
     MDP_DEV RowGrad(const GradArgs& g, int64_t row) {
         const float inv_t = inverse_temperature(g.temperature, g.temperature_s, row);
         m = g.stats[3 * row];
         c = inv_t * kLog2E;
         const float log_s = g.stats[3 * row + 1], h = g.stats[3 * row + 2];
-        log2_s = log_s * kLog2E;
+        log2_s = log_s == -kInf ? 0.0f : log_s * kLog2E;               // a row without allowed entries: p = 0 everywhere
         const int64_t a = g.actions[row];
         action = a >= 0 && a < g.vocab ? (int)a : -1;
         float gl = g.grad_log_prob ? g.grad_log_prob[row] : 0.0f;
@@ -528,12 +532,35 @@ struct RowGrad {
         hot = gl * inv_t;
         a0 = -(gl + ge * h) * inv_t;
         a1 = -ge * kLn2 * inv_t;
+        whole = a0 - a0 == 0.0f && a1 - a1 == 0.0f && log2_s == log2_s;
     }
-    MDP_DEV float operator()(float x, int i) const {
+    MDP_DEV float operator()(float x) const {
+        const float lp = larger(fmaf(x - m, c, -log2_s), -300.0f);
+        return __builtin_amdgcn_exp2f(lp) * fmaf(a1, lp, a0);
+    }
+    MDP_DEV float of_broken(float x) const {
         if (x == -kInf) return 0.0f;
-        const float lp = larger((x - m) * c - log2_s, -300.0f), p = __builtin_amdgcn_exp2f(x != x ? x : lp);
-        float y = p * fmaf(a1, lp, a0);
-        return i == action ? y + hot : y;
+        const float lp = fmaf(x - m, c, -log2_s);
+        return __builtin_amdgcn_exp2f(lp) * fmaf(a1, lp, a0);
+    }
+    // gradients of N entries from entry i0 on, in place
+    template <int N>
+    MDP_DEV void apply(float (&v)[N], int i0) const {
+        const int at = action - i0;
+        const bool here = (unsigned)at < (unsigned)N;  // the action is one of them
+        uint32_t possible = 0;
+        if (here)
+#pragma unroll
+            for (int e = 0; e < N; ++e) possible |= e == at && v[e] != -kInf ? 1u << e : 0u;
+        if (whole)
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = (*this)(v[e]);
+        else
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = of_broken(v[e]);
+        if (here)
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] += possible >> e & 1u ? hot : 0.0f;
     }
 };
 
@@ -553,8 +580,7 @@ __global__ __launch_bounds__(256) void k_grad_short(GradArgs g) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int j = k * G + lane, i0 = j * N - r.shift;
-#pragma unroll
-        for (int e = 0; e < N; ++e) v[k][e] = f(v[k][e], i0 + e);
+        f.apply(v[k], i0);
         if (same && r.full(j)) *(uint4*)(out + i0) = Chunk<T>::of(v[k]).raw;
         else
 #pragma unroll
@@ -567,31 +593,50 @@ __global__ __launch_bounds__(256) void k_grad_short(GradArgs g) {
 // them is still in the caches.
 template <typename T, bool MASK>
 __global__ __launch_bounds__(256) void k_grad_long(GradArgs g) {
-    constexpr int N = Chunk<T>::N;
+    constexpr int N = Chunk<T>::N, B = 4;
     const int64_t row = g.rows - 1 - blockIdx.x / g.pieces;
     const int piece = blockIdx.x % g.pieces, tid = threadIdx.x;
     const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
     T* out = (T*)g.grad + row * g.ld_grad;
     const bool same = ((uintptr_t)out & 15) == ((uintptr_t)r.x & 15);
-    const RowGrad<T> f(g, row);
     const int first = r.full_first(), end = r.full_end();
-#pragma unroll 4
-    for (int j = first + piece * 256 + tid; j < end; j += g.pieces * 256) {
-        const Chunk<T> raw = r.chunk(j);
-        const uint32_t ok = MASK ? r.allowed_chunk(j) : ~0u;
-        const int i0 = j * N - r.shift;
-        float v[N];
+    for (int j0 = first + piece * (256 * B) + tid; j0 < end; j0 += g.pieces * (256 * B)) {
+        Chunk<T> raw[B];
+        uint32_t ok[B];
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = f(ok >> e & 1u ? raw.at(e) : -kInf, i0 + e);
-        if (same) *(uint4*)(out + i0) = Chunk<T>::of(v).raw;
-        else
+        for (int b = 0; b < B; ++b) {
+            const int j = j0 + 256 * b;
+            raw[b] = Chunk<T>::lowest();
+            ok[b] = 0;
+            if (j < end) {
+                raw[b] = r.chunk(j);
+                if (MASK) ok[b] = r.allowed_chunk(j);
+            }
+        }
+        const RowGrad<T> f(g, row);                    // after the loads of the entries are on their way
 #pragma unroll
-            for (int e = 0; e < N; ++e) from_f32(v[e], out[i0 + e]);
+        for (int b = 0; b < B; ++b) {
+            const int j = j0 + 256 * b, i0 = j * N - r.shift;
+            if (j >= end) break;
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = !MASK || (ok[b] >> e & 1u) ? raw[b].at(e) : -kInf;
+            f.apply(v, i0);
+            if (same) *(uint4*)(out + i0) = Chunk<T>::of(v).raw;
+            else
+#pragma unroll
+                for (int e = 0; e < N; ++e) from_f32(v[e], out[i0 + e]);
+        }
     }
     if (piece) return;
     const int head = first ? min(r.V, N - r.shift) : 0, tail = max(head, end * N - r.shift);
     const int i = tid < head ? tid : tail + tid - head;
-    if (i < r.V) from_f32(f(r.entry(i), i), out[i]);
+    if (i < r.V) {
+        const RowGrad<T> f(g, row);
+        float v[1] = {r.entry(i)};
+        f.apply(v, i);
+        from_f32(v[0], out[i]);
+    }
 }
 
 int check_rows(const char* what, const void* logits, int64_t rows, int64_t vocab, int64_t ld, int dtype, const uint8_t* mask,
@@ -632,11 +677,18 @@ extern "C" int mdp_categorical_sample(const mdp_categorical_sample_t* a, void* s
 
 namespace {
 
-// The most chunks that a row of `vocab` entries can touch decides how many lanes hold it; beyond 256 chunks (1024 floats, 2048
-// 16-bit entries) a row is a block's.
+// The most chunks that a row can touch: one more than it fills where rows do not all start on a chunk's boundary.
+template <typename T>
+int most_chunks(const void* logits, int64_t ld, int64_t rows, int vocab) {
+    constexpr int N = Chunk<T>::N;
+    const bool aligned = ((uintptr_t)logits & 15) == 0 && (rows == 1 || ld % N == 0);
+    return (vocab + (aligned ? 0 : N - 1) + N - 1) / N;
+}
+
+// That number decides how many lanes hold a row; beyond 256 chunks (1024 floats, 2048 16-bit entries) a row is a block's.
 template <typename T, bool MASK>
 void launch_evaluate(const EvalArgs& g, hipStream_t s) {
-    const int chunks = (g.vocab + 2 * (Chunk<T>::N - 1)) / Chunk<T>::N;
+    const int chunks = most_chunks<T>(g.logits, g.ld, g.rows, g.vocab);
 #define SHORT(G, K)                                                                                                            \
     if (chunks <= G * K) {                                                                                                     \
         hipLaunchKernelGGL((k_evaluate_short<T, MASK, G, K>), dim3((unsigned)((g.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, s, g); \
@@ -649,7 +701,7 @@ void launch_evaluate(const EvalArgs& g, hipStream_t s) {
 
 template <typename T, bool MASK>
 void launch_grad(GradArgs g, hipStream_t s) {
-    const int chunks = (g.vocab + 2 * (Chunk<T>::N - 1)) / Chunk<T>::N;
+    const int chunks = most_chunks<T>(g.logits, g.ld, g.rows, g.vocab);
 #define SHORT(G, K)                                                                                                        \
     if (chunks <= G * K) {                                                                                                 \
         hipLaunchKernelGGL((k_grad_short<T, MASK, G, K>), dim3((unsigned)((g.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, s, g); \

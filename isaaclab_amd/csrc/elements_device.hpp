@@ -1,6 +1,7 @@
 // Element types of the policy-side kernels (categorical.hip, grad_clip.hip): float, bfloat16 and half in memory, float in registers.
 #pragma once
 #include "mdp_device.hpp"
+#include <type_traits>
 
 namespace mdp {
 
@@ -24,6 +25,10 @@ struct Chunk {
     MDP_DEV float at(int e) const {
         const uint32_t w = e * (int)sizeof(T) / 4 == 0 ? raw.x : e * (int)sizeof(T) / 4 == 1 ? raw.y : e * (int)sizeof(T) / 4 == 2 ? raw.z : raw.w;
         return unpack((T*)nullptr, w, e);
+    }
+    MDP_DEV static Chunk lowest() {                    // -inf in every place
+        const uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, f16>::value ? 0xfc00fc00u : 0xff80ff80u;
+        return Chunk{uint4{w, w, w, w}};
     }
     MDP_DEV static Chunk of(const float (&v)[N]) {
         Chunk c;

@@ -47,26 +47,50 @@ MDP_DEV double block_join(double v, double* red) {
     return v;
 }
 
-// calls f(tensor, first element, elements) for each of this block's chunks: block b of B takes chunks [b C / B, (b + 1) C / B)
-template <class F>
+// calls f(tensor, first element, elements) for each of this block's chunks: block b of B takes chunks [b C / B, (b + 1) C / B),
+// backwards from the last block on if BACK
+template <bool BACK = false, class F>
 MDP_DEV void for_chunks(const Table& t, F&& f) {
-    int64_t c = (int64_t)blockIdx.x * t.chunks / gridDim.x;
-    const int64_t end = (int64_t)(blockIdx.x + 1) * t.chunks / gridDim.x;
-    int i = 0;
-    while (i + 1 < t.n && t.start[i + 1] <= c) ++i;
-    for (; c < end; ++c) {
-        while (t.start[i + 1] <= c) ++i;
-        const int64_t at = (c - t.start[i]) * kChunk, left = t.count[i] - at;
+    const int64_t b = BACK ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    const int first = (int)(b * t.chunks / gridDim.x), end = (int)((b + 1) * t.chunks / gridDim.x);
+    if (first == end) return;
+    int i = 0;                                         // the tensor of the first chunk: the last that starts at or before it
+    const int c0 = BACK ? end - 1 : first;
+    for (int step = 64; step; step >>= 1)
+        if (i + step < t.n && t.start[i + step] <= c0) i += step;
+    for (int k = 0; k < end - first; ++k) {
+        const int c = BACK ? end - 1 - k : first + k;
+        while (BACK ? t.start[i] > c : t.start[i + 1] <= c) i += BACK ? -1 : 1;
+        const int64_t at = (int64_t)(c - t.start[i]) * kChunk, left = t.count[i] - at;
         f(i, at, (int)(left < kChunk ? left : kChunk));
     }
 }
 
-template <int KIND, typename T>
-MDP_DEV double chunk_norm(const T* g, int n, double acc) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const double v = (double)to_f32(g[i]);
-        acc = joined<KIND>(acc, KIND == 2 ? v * v : fabs(v));
+// f(value) for each of this thread's elements of a chunk; 16-byte loads, all of them in flight, where the tensor starts on a
+// 16-byte boundary (chunks then do too)
+template <typename T, class F>
+MDP_DEV void each(const T* g, int n, bool whole, F&& f) {
+    constexpr int N = Chunk<T>::N, B = kChunk / (256 * N);
+    if (whole) {
+        Chunk<T> c[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) c[b].raw = ((const uint4*)g)[b * 256 + threadIdx.x];
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int e = 0; e < N; ++e) f(c[b].at(e));
+    } else {
+        for (int i = threadIdx.x; i < n; i += 256) f(to_f32(g[i]));
     }
+}
+
+template <int KIND, typename T>
+MDP_DEV double chunk_norm(const void* grad, int64_t at, int n, double acc) {
+    const T* g = (const T*)grad + at;
+    each(g, n, n == kChunk && ((uintptr_t)g & 15) == 0, [&](float x) {
+        const double v = (double)x;
+        acc = KIND == 2 ? fma(v, v, acc) : joined<KIND>(acc, fabs(v));
+    });
     return acc;
 }
 
@@ -75,43 +99,76 @@ __global__ __launch_bounds__(256) void k_grad_partial(Table t, double* __restric
     __shared__ double red[4];
     double acc = 0.0;
     for_chunks(t, [&](int i, int64_t at, int n) {
-        if (t.dtype[i] == MDP_DTYPE_F32) acc = chunk_norm<KIND>((const float*)t.grad[i] + at, n, acc);
-        else if (t.dtype[i] == MDP_DTYPE_BF16) acc = chunk_norm<KIND>((const bf16*)t.grad[i] + at, n, acc);
-        else acc = chunk_norm<KIND>((const f16*)t.grad[i] + at, n, acc);
+        if (t.dtype[i] == MDP_DTYPE_F32) acc = chunk_norm<KIND, float>(t.grad[i], at, n, acc);
+        else if (t.dtype[i] == MDP_DTYPE_BF16) acc = chunk_norm<KIND, bf16>(t.grad[i], at, n, acc);
+        else acc = chunk_norm<KIND, f16>(t.grad[i], at, n, acc);
     });
     acc = block_join<KIND>(acc, red);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
+// every thread of a block gets what the partial sums join to
 template <int KIND>
-__global__ __launch_bounds__(256) void k_grad_finish(const double* __restrict__ partial, int64_t n, double max_norm,
-                                                     float* __restrict__ norm, float* __restrict__ factor) {
-    __shared__ double red[4];
+MDP_DEV double joined_partials(const double* __restrict__ partial, int n, double* red) {
     double acc = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 256) acc = joined<KIND>(acc, partial[i]);
-    acc = block_join<KIND>(acc, red);
+    for (int i = threadIdx.x; i < n; i += 256) acc = joined<KIND>(acc, partial[i]);
+    return block_join<KIND>(acc, red);
+}
+
+// the norm of the partial sums, and what they join to in their place: for a call that only wants the norm, or has so many
+// tensors that the partial sums are more than every block should read
+template <int KIND>
+__global__ __launch_bounds__(256) void k_grad_finish(const double* __restrict__ partial, int n, double* __restrict__ all,
+                                                     float* __restrict__ norm) {
+    __shared__ double red[4];
+    const double acc = joined_partials<KIND>(partial, n, red);
     if (threadIdx.x) return;
-    if (KIND == 2) acc = sqrt(acc);
-    *norm = (float)acc;
-    const double f = max_norm / (acc + 1e-6);
-    if (factor) *factor = f != f || f < 1.0 ? (float)f : 1.0f;
+    *all = acc;
+    *norm = (float)(KIND == 2 ? sqrt(acc) : acc);
 }
 
 template <typename T, typename U>
-MDP_DEV void chunk_scale(const T* g, U* out, int n, float f) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) from_f32(to_f32(g[i]) * f, out[i]);
+MDP_DEV void chunk_scale(const void* grad, void* to, int64_t at, int n, float f) {
+    constexpr int N = Chunk<T>::N, B = kChunk / (256 * N), M = Chunk<U>::N;
+    const T* g = (const T*)grad + at;
+    U* out = (U*)to + at;
+    if (n == kChunk && (((uintptr_t)g | (uintptr_t)out) & 15) == 0) {
+        Chunk<T> c[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) c[b].raw = ((const uint4*)g)[b * 256 + threadIdx.x];
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int h = 0; h < N / M; ++h) {
+                float v[M];
+#pragma unroll
+                for (int e = 0; e < M; ++e) v[e] = c[b].at(h * M + e) * f;
+                ((uint4*)out)[(b * 256 + threadIdx.x) * (N / M) + h] = Chunk<U>::of(v).raw;
+            }
+    } else {
+        for (int i = threadIdx.x; i < n; i += 256) from_f32(to_f32(g[i]) * f, out[i]);
+    }
 }
 
-__global__ __launch_bounds__(256) void k_grad_scale(Table t, const float* __restrict__ factor) {
-    const float f = *factor;
-    for_chunks(t, [&](int i, int64_t at, int n) {
+// Every block joins the partial sums by itself (at most 1024 of them, from the caches): no launch between the two.  Chunks are
+// taken from the last one back, so that what the norm read last, and is still in the caches, comes first.
+template <int KIND>
+__global__ __launch_bounds__(256) void k_grad_scale(Table t, const double* __restrict__ partial, int partials, double max_norm,
+                                                    float* __restrict__ norm) {
+    __shared__ double red[4];
+    double total = joined_partials<KIND>(partial, partials, red);
+    total = KIND == 2 ? sqrt(total) : total;
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
+    const double ratio = max_norm / (total + 1e-6);
+    const float f = ratio != ratio || ratio < 1.0 ? (float)ratio : 1.0f;
+    for_chunks<true>(t, [&](int i, int64_t at, int n) {
         if (t.out[i] == t.grad[i] && f == 1.0f) return;
         const int from = t.dtype[i], to = t.out_dtype[i];
-        if (from == MDP_DTYPE_F32) chunk_scale((const float*)t.grad[i] + at, (float*)t.out[i] + at, n, f);
-        else if (from == MDP_DTYPE_BF16 && to == from) chunk_scale((const bf16*)t.grad[i] + at, (bf16*)t.out[i] + at, n, f);
-        else if (from == MDP_DTYPE_BF16) chunk_scale((const bf16*)t.grad[i] + at, (float*)t.out[i] + at, n, f);
-        else if (to == from) chunk_scale((const f16*)t.grad[i] + at, (f16*)t.out[i] + at, n, f);
-        else chunk_scale((const f16*)t.grad[i] + at, (float*)t.out[i] + at, n, f);
+        if (from == MDP_DTYPE_F32) chunk_scale<float, float>(t.grad[i], t.out[i], at, n, f);
+        else if (from == MDP_DTYPE_BF16 && to == from) chunk_scale<bf16, bf16>(t.grad[i], t.out[i], at, n, f);
+        else if (from == MDP_DTYPE_BF16) chunk_scale<bf16, float>(t.grad[i], t.out[i], at, n, f);
+        else if (to == from) chunk_scale<f16, f16>(t.grad[i], t.out[i], at, n, f);
+        else chunk_scale<f16, float>(t.grad[i], t.out[i], at, n, f);
     });
 }
 
@@ -195,19 +252,18 @@ void for_tables(const mdp_grad_t* g, int64_t n, F&& f) {
         else { constexpr int K = 0; launch; }                   \
     } while (0)
 
-void launch_norm(const mdp_grad_t* g, int64_t n, int kind, double max_norm, double* workspace, float* norm, float* factor,
-                 hipStream_t s) {
+int64_t launch_partials(const mdp_grad_t* g, int64_t n, int kind, double* partial, hipStream_t s) {
     int64_t partials = 0;
     for_tables(g, n, [&](const Table& t, unsigned blocks) {
-        BY_KIND(kind, hipLaunchKernelGGL(k_grad_partial<K>, dim3(blocks), dim3(256), 0, s, t, workspace + 1 + partials));
+        BY_KIND(kind, hipLaunchKernelGGL(k_grad_partial<K>, dim3(blocks), dim3(256), 0, s, t, partial + partials));
         partials += blocks;
     });
-    BY_KIND(kind, hipLaunchKernelGGL(k_grad_finish<K>, dim3(1), dim3(256), 0, s, workspace + 1, partials, max_norm, norm, factor));
+    return partials;
 }
 
 }  // namespace
 
-// one word for the factor, then the partial sums of each table
+// the partial sums of each table, and what they join to
 extern "C" int64_t mdp_grad_workspace(int64_t num_grads) {
     const int64_t n = num_grads > 0 ? num_grads : 0;
     return 1 + kBlocks * ((n + kTable - 1) / kTable);
@@ -216,7 +272,9 @@ extern "C" int64_t mdp_grad_workspace(int64_t num_grads) {
 extern "C" int mdp_grad_norm(const mdp_grad_t* grads, int64_t num_grads, int norm_kind, double* workspace, float* norm,
                              void* stream) {
     if (int rc = check_grads(grads, num_grads, norm_kind, workspace, norm, false)) return rc;
-    launch_norm(grads, num_grads, norm_kind, 0.0, workspace, norm, nullptr, as_stream(stream));
+    hipStream_t s = as_stream(stream);
+    const int partials = (int)launch_partials(grads, num_grads, norm_kind, workspace, s);
+    BY_KIND(norm_kind, hipLaunchKernelGGL(k_grad_finish<K>, dim3(1), dim3(256), 0, s, workspace, partials, workspace + partials, norm));
     MDP_LAUNCH_CHECK();
     return MDP_OK;
 }
@@ -227,10 +285,13 @@ extern "C" int mdp_grad_clip(const mdp_grad_t* grads, int64_t num_grads, int nor
     MDP_REQUIRE(max_norm >= 0.0, "grad_clip: max_norm %g is negative or NaN", max_norm);
     if (int rc = check_overlap(grads, num_grads)) return rc;
     hipStream_t s = as_stream(stream);
-    float* factor = (float*)workspace;
-    launch_norm(grads, num_grads, norm_kind, max_norm, workspace, norm, factor, s);
+    const int partials = (int)launch_partials(grads, num_grads, norm_kind, workspace, s);
+    const bool joined = partials == 0 || partials > kBlocks;
+    if (joined)
+        BY_KIND(norm_kind, hipLaunchKernelGGL(k_grad_finish<K>, dim3(1), dim3(256), 0, s, workspace, partials, workspace + partials, norm));
     for_tables(grads, num_grads, [&](const Table& t, unsigned blocks) {
-        hipLaunchKernelGGL(k_grad_scale, dim3(blocks), dim3(256), 0, s, t, factor);
+        BY_KIND(norm_kind, hipLaunchKernelGGL(k_grad_scale<K>, dim3(blocks), dim3(256), 0, s, t, workspace + (joined ? partials : 0),
+                                              joined ? 1 : partials, max_norm, joined ? nullptr : norm));
     });
     MDP_LAUNCH_CHECK();
     return MDP_OK;

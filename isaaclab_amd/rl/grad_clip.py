@@ -8,6 +8,7 @@ import torch
 
 from .. import _lib as L
 
+_DTYPES = L.DTYPES
 _KINDS = {2.0: 2, 1.0: 1, float("inf"): 0}
 
 
@@ -45,32 +46,57 @@ def _as_list(tensors) -> list:
     return [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
 
 
+def _table(grads: list, outs: list | None) -> tuple[array, int]:
+    """(``mdp_grad_t`` table: two pointers, the count and the two element types of each, as 64-bit words; device index)."""
+    try:
+        index = grads[0].get_device()
+        kinds = [_DTYPES[t.dtype] for t in grads]
+        plain = all([t.is_contiguous() for t in grads])
+        if outs is None:
+            outs, to = grads, kinds
+        else:
+            to = [_DTYPES[t.dtype] for t in outs]
+            plain = (plain and all([t.is_contiguous() for t in outs]) and [t.shape for t in outs] == [t.shape for t in grads]
+                     and all([o == k or o == 0 for o, k in zip(to, kinds)]) and {t.get_device() for t in outs} == {index})
+        plain = plain and index >= 0 and {t.get_device() for t in grads} == {index}
+    except (AttributeError, KeyError, RuntimeError):
+        plain = False
+    if not plain:                            # something to refuse, or strides that take a closer look
+        _check_all(grads, outs or grads)
+        index = grads[0].get_device()
+        kinds, to = [_DTYPES[t.dtype] for t in grads], [_DTYPES[t.dtype] for t in outs or grads]
+        outs = outs or grads
+    words = [w for g, o, k, u in zip(grads, outs, kinds, to) for w in (g.data_ptr(), o.data_ptr(), g.numel(), k | u << 32)]
+    return array("q", words), index
+
+
+def _check_all(grads: list, outs: list):
+    device = grads[0].device if isinstance(grads[0], torch.Tensor) else None
+    for g, o in zip(grads, outs):
+        _check(g, device, "gradient")
+        if o is g:
+            continue
+        _check(o, device, "out")
+        if o.dtype != g.dtype and o.dtype != torch.float32:
+            raise ValueError(f"out must be of its gradient's type or float32, got {o.dtype} for {g.dtype}")
+        if o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
+            raise ValueError(f"out must have its gradient's shape and strides: {tuple(o.shape)} {o.stride()} for "
+                             f"{tuple(g.shape)} {g.stride()}")
+
+
 def _launch(grads: list, outs: list | None, kind: int, max_norm: float | None) -> torch.Tensor:
     if not grads:
         return torch.zeros((), dtype=torch.float32)
-    first = grads[0]
-    device = first.device if isinstance(first, torch.Tensor) else None
-    words = []
-    for g, o in zip(grads, outs or grads):
-        _check(g, device, "gradient")
-        if o is not g:
-            _check(o, device, "out")
-            if o.dtype != g.dtype and o.dtype != torch.float32:
-                raise ValueError(f"out must be of its gradient's type or float32, got {o.dtype} for {g.dtype}")
-            if o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
-                raise ValueError(f"out must have its gradient's shape and strides: {tuple(o.shape)} {o.stride()} for "
-                                 f"{tuple(g.shape)} {g.stride()}")
-        words += (g.data_ptr(), o.data_ptr(), g.numel(), L.DTYPES[g.dtype] | L.DTYPES[o.dtype] << 32)
-    table = array("q", words)                # mdp_grad_t[n]: two pointers, the count, the two element types
-    n = len(grads)
+    table, index = _table(grads, outs)
+    n, device = len(grads), grads[0].device
     workspace = torch.empty(L.lib.mdp_grad_workspace(n), dtype=torch.float64, device=device)
     norm = torch.empty((), dtype=torch.float32, device=device)
     with L.on_device(device):
         if max_norm is None:
-            rc = L.lib.mdp_grad_norm(table.buffer_info()[0], n, kind, workspace.data_ptr(), norm.data_ptr(), L.stream(device))
+            rc = L.lib.mdp_grad_norm(table.buffer_info()[0], n, kind, workspace.data_ptr(), norm.data_ptr(), L.stream(index))
         else:
             rc = L.lib.mdp_grad_clip(table.buffer_info()[0], n, kind, max_norm, workspace.data_ptr(), norm.data_ptr(),
-                                     L.stream(device))
+                                     L.stream(index))
     L.check(rc)
     return norm
 

@@ -48,221 +48,6 @@ MDP_DEV double exp2_neg(double t) {
     return __builtin_ldexp(p, (int)n);
 }
 
-// -- reductions: every lane gets the result; sums in a fixed order -----------------------------------------------------
-MDP_DEV double wave_sum(double v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-MDP_DEV int64_t wave_sum(int64_t v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((long long)v, o);
-    return v;
-}
-MDP_DEV float wave_max(float v) {
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
-MDP_DEV double wave_scan(double v) {                 // inclusive
-    const int lane = threadIdx.x & 63;
-    for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(v, o);
-        if (lane >= o) v += up;
-    }
-    return v;
-}
-
-struct SampleArgs {
-    const void* logits; int64_t ld;
-    const uint8_t* mask; int64_t ld_mask;
-    int vocab;
-    const float* temperature; const int* top_k; const float* top_p; const float* min_p;
-    float temperature_s; int top_k_s; float top_p_s; float min_p_s;
-    const float* u; const unsigned long long* state;
-    int64_t* actions; float* log_prob;
-};
-
-constexpr uint32_t kStream = 0x43415447u;
-
-template <int THREADS>
-struct Block {
-    static constexpr int W = THREADS / 64;
-    struct Shared { double d[W]; int64_t n[W]; float f[W]; int bad[W]; };
-    Shared* s;
-    MDP_DEV double sum(double v) {
-        v = wave_sum(v);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) s->d[threadIdx.x >> 6] = v;
-        __syncthreads();
-        double r = 0.0;
-        for (int w = 0; w < W; ++w) r += s->d[w];
-        return r;
-    }
-    MDP_DEV int64_t sum(int64_t v) {
-        v = wave_sum(v);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) s->n[threadIdx.x >> 6] = v;
-        __syncthreads();
-        int64_t r = 0;
-        for (int w = 0; w < W; ++w) r += s->n[w];
-        return r;
-    }
-    MDP_DEV float max(float v) {
-        v = wave_max(v);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) s->f[threadIdx.x >> 6] = v;
-        __syncthreads();
-        float r = s->f[0];
-        for (int w = 1; w < W; ++w) r = fmaxf(r, s->f[w]);
-        return r;
-    }
-};
-
-// One block draws one row.  Each question about the row (its maximum, how many entries and how much mass lie at or above a
-// key, where the running mass passes u W) is one pass over it.
-template <typename T, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_sample_row(SampleArgs g) {
-    using B = Block<THREADS>;
-    __shared__ typename B::Shared sh;
-    __shared__ double wave_mass[B::W];
-    __shared__ int64_t wave_level[B::W];
-    B b{&sh};
-    const int64_t row = blockIdx.x;
-    const int V = g.vocab, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const T* x = (const T*)g.logits + row * g.ld;
-    const uint8_t* mask = g.mask ? g.mask + row * g.ld_mask : nullptr;
-    const auto load = [&](int i) { return mask && !mask[i] ? -kInf : to_f32(x[i]); };
-
-    const float temp = g.temperature ? g.temperature[row] : g.temperature_s;
-    float m = -kInf;
-    int64_t bad = 0;
-    for (int i = tid; i < V; i += THREADS) {
-        const float v = load(i);
-        bad |= v != v || v == kInf;
-        m = fmaxf(m, v);
-    }
-    m = b.max(m);
-    bad = b.sum(bad);
-    if (bad || !(temp >= 0.0f)) {                      // no distribution
-        if (tid == 0) { g.actions[row] = -1; g.log_prob[row] = __builtin_nanf(""); }
-        return;
-    }
-    if (m == -kInf) {                                  // nothing to choose from
-        if (tid == 0) { g.actions[row] = -1; g.log_prob[row] = 0.0f; }
-        return;
-    }
-    const bool greedy = temp == 0.0f;
-    const double c = greedy ? 0.0 : 1.4426950408889634 / (double)temp;
-    const auto weight = [&](float v) { return v == -kInf ? 0.0 : exp2_neg(((double)v - (double)m) * c); };
-    const auto count_from = [&](uint32_t k) {
-        int64_t n = 0;
-        for (int i = tid; i < V; i += THREADS) n += key_of(load(i)) >= k;
-        return b.sum(n);
-    };
-    const auto mass_from = [&](uint32_t k) {
-        double n = 0.0;
-        for (int i = tid; i < V; i += THREADS) { const float v = load(i); n += key_of(v) >= k ? weight(v) : 0.0; }
-        return b.sum(n);
-    };
-
-    // the prefix {key > tau} and the first `room` entries of key tau
-    const uint32_t top = key_of(m), lowest = key_of(-kInf) + 1u;
-    uint32_t tau = greedy ? top : lowest;
-    int64_t room = greedy ? 1 : V;
-    float p = g.top_p ? g.top_p[row] : g.top_p_s, mp = g.min_p ? g.min_p[row] : g.min_p_s;
-    const int64_t k = g.top_k ? g.top_k[row] : g.top_k_s;
-    if (!greedy) {
-        if (k > 0 && k < V && count_from(lowest) > k) {
-            uint32_t lo = lowest, hi = top;
-            while (lo < hi) {
-                const uint32_t mid = lo + (hi - lo + 1u) / 2u;
-                if (count_from(mid) >= k) lo = mid; else hi = mid - 1u;
-            }
-            tau = lo;
-            room = k - count_from(tau + 1u);
-        }
-        if (p < 1.0f) {
-            p = p > 0.0f ? p : 0.0f;
-            const double above = mass_from(tau + 1u);
-            int64_t level = count_from(tau) - count_from(tau + 1u);
-            if (level > room) level = room;
-            const double aim = (double)p * (above + (double)level * weight(of_key(tau)));
-            uint32_t lo = tau, hi = top;
-            while (lo < hi) {
-                const uint32_t mid = lo + (hi - lo + 1u) / 2u;
-                if (mass_from(mid) >= aim) lo = mid; else hi = mid - 1u;
-            }
-            // entries of the level: each that has less than `aim` before it
-            const double need = (aim - mass_from(lo + 1u)) / weight(of_key(lo));
-            int64_t r = need < 1.0 ? 1 : need > (double)V ? V : (int64_t)__builtin_ceil(need);
-            room = lo == tau && room < r ? room : r;
-            tau = lo;
-        }
-    }
-    mp = mp > 0.0f ? (mp < 1.0f ? mp : 1.0f) : 0.0f;
-
-    // each wave owns a contiguous piece of the row, so running counts and masses follow the index
-    const int piece = ((V + THREADS - 1) / THREADS) * 64, first = wave * piece, last = min(V, first + piece);
-    int64_t level = 0;
-    for (int i = first + lane; i < last; i += 64) level += key_of(load(i)) == tau;
-    level = wave_sum(level);
-    if (lane == 0) wave_level[wave] = level;
-    __syncthreads();
-    int64_t rank0 = 0;
-    for (int w = 0; w < wave; ++w) rank0 += wave_level[w];
-    const auto walk = [&](auto&& visit) {              // visit(i, weight of entry i if it is kept): uniform over the wave
-        int64_t rank = rank0;
-        for (int i0 = first; i0 < last; i0 += 64) {
-            const int i = i0 + lane;
-            const float v = i < last ? load(i) : -kInf;
-            const uint32_t key = key_of(v);
-            const uint64_t eq = __ballot(key == tau);
-            const int64_t mine = rank + __popcll(eq & ((1ull << lane) - 1ull));
-            rank += __popcll(eq);
-            double w = key > tau || (key == tau && mine < room) ? weight(v) : 0.0;
-            w = w >= (double)mp ? w : 0.0;
-            if (visit(i, w)) return;
-        }
-    };
-    double mass = 0.0;
-    walk([&](int, double w) { mass += w; return false; });
-    mass = wave_sum(mass);
-    if (lane == 0) wave_mass[wave] = mass;
-    __syncthreads();
-    double total = 0.0;
-    for (int w = 0; w < B::W; ++w) total += wave_mass[w];
-    float u = 0.0f;
-    if (g.u) u = g.u[row];
-    else u = u01(rng4(g.state[0], g.state[1], kStream, (uint64_t)row).x);
-    u = u > 0.0f ? (u < 0.99999994f ? u : 0.99999994f) : 0.0f;
-    const double aim = (double)u * total;
-    int target = -1;
-    double before = 0.0, run = 0.0;
-    for (int w = 0; w < B::W; ++w) {
-        if (wave_mass[w] > 0.0 && run <= aim) { target = w; before = run; }   // the last one that begins at or below the aim
-        run += wave_mass[w];
-    }
-    if (wave != target) return;
-    int found = -1;
-    double found_w = 0.0;
-    walk([&](int i, double w) {
-        const double upto = before + wave_scan(w);
-        const uint64_t over = __ballot(upto > aim && w > 0.0), some = __ballot(w > 0.0);
-        // rounding may leave the aim at the very end of the piece: the last entry with mass is the answer then
-        if (some) {
-            const int l = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
-            found = __shfl(i, l);
-            found_w = __shfl(w, l);
-        }
-        before = __shfl(upto, 63);
-        return over != 0ull;
-    });
-    if (lane == 0) {
-        g.actions[row] = found;
-        g.log_prob[row] = greedy ? 0.0f : (float)log(found_w / total);
-    }
-}
-
-__global__ void k_state_advance(unsigned long long* state) { state[1] += 1ull; }
-
 // -- rows ---------------------------------------------------------------------------------------------------------------
 // A row as the 16-byte chunks of memory that it touches: chunk j holds entries j N - shift .. j N - shift + N - 1, of which
 // the first and the last chunk may hold some that are not the row's.  Those are never read: an edge chunk is read entry by
@@ -347,6 +132,711 @@ template <int G>
 MDP_DEV float group_max(float v) { return over_group<G>(v, [](float a, float b) { return larger(a, b); }); }
 template <int G>
 MDP_DEV float group_sum(float v) { return over_group<G>(v, [](float a, float b) { return a + b; }); }
+
+template <int G>
+MDP_DEV double group_sum(double v) {
+    for (int o = 1; o < G; o <<= 1) v += __shfl_xor(v, o);
+    return v;
+}
+template <int G>
+MDP_DEV int group_sum(int v) {
+    for (int o = 1; o < G; o <<= 1) v += __shfl_xor(v, o);
+    return v;
+}
+// sum over the lanes of the group up to and with this one
+template <int G, typename V>
+MDP_DEV V group_scan(V v) {
+    const int lane = threadIdx.x % G;
+    for (int o = 1; o < G; o <<= 1) {
+        const V up = __shfl_up(v, o);
+        if (lane >= o) v += up;
+    }
+    return v;
+}
+
+// -- drawing ------------------------------------------------------------------------------------------------------------
+// Everything that decides is in 64 bits, which cost what 32 bits cost on this chip's vector units: weights, their sums and the
+// comparisons with u W and p S.  Sums in 32 bits only ever bound what has to be looked at.
+struct SampleArgs {
+    const void* logits; int64_t ld;
+    const uint8_t* mask; int64_t ld_mask;
+    int vocab; int64_t rows;
+    const float* temperature; const int* top_k; const float* top_p; const float* min_p;
+    float temperature_s; int top_k_s; float top_p_s; float min_p_s;
+    const float* u; const unsigned long long* state;
+    int64_t* actions; float* log_prob;
+};
+
+constexpr uint32_t kStream = 0x43415447u;
+
+// A row's settings.  Temperature 0 is one entry of the largest logit, with weights that are 1 there and 0 elsewhere.
+struct Settings {
+    double c;                                          // log2(e) / T; a NaN for a temperature that is negative or NaN
+    int k;                                             // 0: no limit
+    double p, mp;                                      // p = 1, mp = 0: no limit
+    double u;
+    MDP_DEV Settings(const SampleArgs& g, int64_t row) {
+        const float t = g.temperature ? g.temperature[row] : g.temperature_s;
+        k = g.top_k ? g.top_k[row] : g.top_k_s;
+        float pf = g.top_p ? g.top_p[row] : g.top_p_s, mf = g.min_p ? g.min_p[row] : g.min_p_s;
+        if (k < 0) k = 0;
+        p = pf < 1.0f ? (pf > 0.0f ? (double)pf : 0.0) : 1.0;
+        mp = mf > 0.0f ? (mf < 1.0f ? (double)mf : 1.0) : 0.0;
+        c = 1.4426950408889634 / (double)t;
+        c = c > 1e-300 ? c : 1e-300;                   // infinite temperature: -inf * c stays -inf
+        if (t == 0.0f) { c = 1e300; k = 1; p = 1.0; mp = 0.0; }
+        if (!(t >= 0.0f)) c = __builtin_nan("");
+        float uf = g.u ? g.u[row] : u01(rng4(g.state[0], g.state[1], kStream, (uint64_t)row).x);
+        u = uf > 0.0f ? (uf < 0.99999994f ? (double)uf : 0.99999994039535522) : 0.0;
+    }
+    MDP_DEV float c32() const { return (float)fmax(fmin(c, 1e30), 1e-30); }     // -inf * c and 0 * c stay what they are
+    MDP_DEV bool all() const { return k == 0 && p == 1.0 && mp == 0.0; }
+    MDP_DEV double weight(float x, float m) const { return exp2_neg(((double)x - (double)m) * c); }
+};
+
+// Border of what is kept: entries above tau, and the first `room` of the `level` entries equal to it.
+struct Border {
+    float tau;
+    int room, level;
+    double above;                                      // mass above tau
+    int count;                                         // entries above tau
+};
+
+MDP_DEV float next_above(float x) { return of_key(key_of(x) + 1u); }
+
+// The largest entry tau with reaches(count, mass) of the entries >= tau, which has to hold for the lowest entry and grow with
+// count and mass.  measure(P) = {count, mass} of the entries >= P, the same for all who search together; below(P) = the largest
+// entry < P.  [lo, hi) always holds the answer: halved by value -- first about where the weights end -- and by key once values
+// stop narrowing it, until one entry or one value is left in it.
+struct Measure { int count; double mass; };
+template <class M, class B, class R, class Any>
+MDP_DEV Border search(float m, double c, int allowed, M&& measure, B&& below, R&& reaches, Any&& any) {
+    float lo = -__FLT_MAX__, hi = next_above(m);
+    Measure at_lo{allowed, 0.0}, at_hi{0, 0.0};
+    const float first = (float)((double)m - 60.0 / c);
+    for (int it = 0;; ++it) {
+        const bool busy = at_lo.count - at_hi.count > 1 && next_above(lo) < hi;
+        if (!any(busy)) break;
+        float mid = it == 0 ? first : 0.5f * lo + 0.5f * hi;
+        if (it > 24 || !(mid > lo && mid < hi)) mid = of_key(key_of(lo) + (key_of(hi) - key_of(lo)) / 2u);
+        const Measure q = measure(mid);
+        if (busy) {
+            if (reaches(q)) { lo = mid; at_lo = q; }
+            else { hi = mid; at_hi = q; }
+        }
+    }
+    return Border{below(hi), 0, at_lo.count - at_hi.count, at_hi.mass, at_hi.count};
+}
+
+// The border that k and p draw together.
+template <class M, class B, class Any>
+MDP_DEV Border find_border(const Settings& s, float m, int allowed, double total, M&& measure, B&& below, Any&& any) {
+    Border b{-__FLT_MAX__, 0x7fffffff, 0, 0.0, 0};
+    const bool by_k = s.k > 0 && s.k < allowed;
+    double held = total;                               // mass of the first k
+    if (any(by_k)) {
+        Border q = search(m, s.c, allowed, measure, below, [&](Measure x) { return x.count >= s.k; }, [&](bool busy) { return any(by_k && busy); });
+        if (by_k) {
+            b = q;
+            b.room = s.k - q.count;
+            held = q.above + (double)b.room * s.weight(q.tau, m);
+        }
+    }
+    const bool by_p = s.p < 1.0;
+    if (any(by_p)) {
+        const double aim = s.p * held;
+        Border q = search(m, s.c, allowed, measure, below, [&](Measure x) { return x.mass >= aim; }, [&](bool busy) { return any(by_p && busy); });
+        if (by_p) {
+            // of the level those that have less than the aim before them, one at least
+            const double need = (aim - q.above) / s.weight(q.tau, m);
+            q.room = need < 1.0 ? 1 : need < (double)q.level ? (int)__builtin_ceil(need) : q.level;
+            if (by_k && !(q.tau > b.tau)) { q = b.room < q.room || q.tau < b.tau ? b : q; }
+            b = q;
+        }
+    }
+    return b;
+}
+
+// Rows of up to G K chunks, 16 entries a lane: G lanes of a wave hold a row and its weights in registers.  A question about the row
+// is a sum over 16 registers and one over G lanes.  Groups of a wave go through their loops together until the last is done.
+template <typename T, bool MASK, int G, int K>
+__global__ __launch_bounds__(256) void k_sample_short(SampleArgs g) {
+    constexpr int N = Chunk<T>::N;
+    const int64_t mine = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t row = mine < g.rows ? mine : g.rows - 1;             // lanes without a row of their own repeat the last
+    const int lane = threadIdx.x % G, at = threadIdx.x & 63;
+    const uint64_t group = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1ull)) << (at - lane);
+    const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
+    float x[K][N];
+#pragma unroll
+    for (int k = 0; k < K; ++k) r.template load<MASK>(k * G + lane, x[k]);
+    const Settings s(g, row);
+    float m = -kInf;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            x[k][e] += 0.0f;                                           // one zero
+            m = larger(x[k][e], m);
+        }
+    m = group_max<G>(m);
+    const bool empty = m == -kInf;
+    double w[K][N], total = 0.0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            w[k][e] = s.weight(x[k][e], empty ? 0.0f : m);
+            total += w[k][e];
+        }
+    total = group_sum<G>(total);
+    const bool good = total > 0.0 && !empty;                           // false for a NaN too
+    const auto any = [&](bool v) { return __any(v && good) != 0; };
+    if (any(!s.all())) {
+        int allowed = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < N; ++e) allowed += x[k][e] > -kInf;
+        allowed = group_sum<G>(allowed);
+        const Border b = find_border(s, m, allowed, total,
+            [&](float from) {
+                Measure q{0, 0.0};
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) {
+                        const bool in = x[k][e] >= from;
+                        q.count += in;
+                        q.mass += in ? w[k][e] : 0.0;
+                    }
+                return Measure{group_sum<G>(q.count), group_sum<G>(q.mass)};
+            },
+            [&](float under) {
+                float v = -kInf;
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v = x[k][e] < under ? larger(x[k][e], v) : v;
+                return group_max<G>(v);
+            }, any);
+        const bool ranked = b.room < b.level;                          // only some of the level stay, by lowest index
+        int rank0 = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            int rank = rank0;
+            if (any(ranked)) {
+                int equal = 0;
+#pragma unroll
+                for (int e = 0; e < N; ++e) equal += x[k][e] == b.tau;
+                const int upto = group_scan<G>(equal);
+                rank = rank0 + upto - equal;
+                rank0 += __shfl(upto, at - lane + G - 1);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const bool equal = x[k][e] == b.tau;
+                const bool keep = (x[k][e] > b.tau || (equal && (!ranked || rank < b.room))) && w[k][e] >= s.mp;
+                rank += equal;
+                w[k][e] = keep ? w[k][e] : 0.0;
+            }
+        }
+    }
+    // masses by chunk index; the chunk row k that holds the aim, the lane in it, the entry in that
+    double part[K], mass = 0.0, sums[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        part[k] = 0.0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) part[k] += w[k][e];
+        sums[k] = group_sum<G>(part[k]);
+        mass += sums[k];
+    }
+    const double aim = s.u * mass;
+    double before = 0.0, run = 0.0;
+    int pick = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (sums[k] > 0.0 && run <= aim) { pick = k; before = run; }
+        run += sums[k];
+    }
+    double v[N], own = 0.0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = 0.0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (k == pick) {
+            own = part[k];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = w[k][e];
+        }
+    const double upto = before + group_scan<G>(own);
+    const uint64_t over = __ballot(own > 0.0 && upto > aim) & group, some = __ballot(own > 0.0) & group;
+    // rounding may leave the aim at the end of the last mass: its lane, and its last entry, then
+    const int winner = over ? __ffsll((unsigned long long)over) - 1 : some ? 63 - __clzll((long long)some) : at - lane;
+    if (at != winner || mine >= g.rows) return;
+    double sum = upto - own, found_w = 1.0;
+    int found = -1;
+    bool open = true;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        sum += v[e];
+        if (open && v[e] > 0.0) {
+            found = (pick * G + lane) * N - r.shift + e;
+            found_w = v[e];
+            open = !(sum > aim);
+        }
+    }
+    g.actions[mine] = good ? found : -1;
+    g.log_prob[mine] = good ? (float)log(found_w / mass) : empty && s.c == s.c ? 0.0f : __builtin_nanf("");
+}
+
+// Longer rows: a block a row.  Each wave owns a contiguous piece of the row, so that running sums follow the index; of it every
+// lane holds up to H chunks in registers, and what does not fit is read again for each question.
+//
+// A question over a long row is dear (131072 bfloat16 entries: 9 us of a CU in 32 bits), so what k, p and min_p keep is looked for
+// among few candidates: the threads' own largest entries are a part of the row, so a value above which THEY already are k, or
+// already hold a share p of the row's mass, is not above the border.  The entries from there on -- a few more than are kept -- are
+// gathered in index order, sorted, and everything exact happens on them.  Where no such value exists or too many entries lie above
+// it (flat rows), the border is searched over the whole row.
+template <typename T, bool MASK, int THREADS, int H>
+struct LongRow {
+    static constexpr int N = Chunk<T>::N, W = THREADS / 64;
+    struct Shared {
+        double d[W + 1];
+        int n[W + 1];
+        float f[W];
+        union {
+            struct { float top[THREADS]; } maxima;
+            struct { uint64_t key[THREADS]; float x[THREADS]; } list;
+        };
+        float bound;
+        int found, last;
+    };
+    const Row<T> r;
+    Shared& sh;
+    const int tid, lane, wave, steps, first, end;      // chunks of this wave: first + 64 step + lane < end
+    Chunk<T> held[H];
+    float m;
+
+    MDP_DEV LongRow(const SampleArgs& g, int64_t row, Shared& shared)
+        : r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row), sh(shared), tid(threadIdx.x), lane(threadIdx.x & 63),
+          wave(threadIdx.x >> 6), steps((r.chunks() + THREADS - 1) / THREADS), first(wave * steps * 64),
+          end(min(first + steps * 64, r.chunks())) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) held[h] = chunk(h);
+    }
+    MDP_DEV Chunk<T> chunk(int step) const {
+        const int j = first + 64 * step + lane;
+        if (step >= steps || j >= end) return Chunk<T>::lowest();
+        if (!MASK && r.full(j)) return r.chunk(j);
+        float v[N];
+        r.template load<MASK>(j, v);
+        return Chunk<T>::of(v);
+    }
+    // f(step, entries) for each of this thread's chunks
+    template <class F>
+    MDP_DEV void each(F&& f) const {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            if (h < steps) {
+                float v[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = held[h].at(e);
+                f(h, v);
+            }
+            __builtin_amdgcn_sched_barrier(0);         // one chunk's arithmetic at a time: all of them at once would not fit the registers
+        }
+        for (int h = H; h < steps; ++h) {
+            const Chunk<T> q = chunk(h);
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = q.at(e);
+            f(h, v);
+        }
+    }
+    MDP_DEV double block_sum(double v) {
+        v = group_sum<64>(v);
+        __syncthreads();
+        if (lane == 0) sh.d[wave] = v;
+        __syncthreads();
+        double t = 0.0;
+        for (int w = 0; w < W; ++w) t += sh.d[w];
+        return t;
+    }
+    MDP_DEV int block_sum(int v) {
+        v = group_sum<64>(v);
+        __syncthreads();
+        if (lane == 0) sh.n[wave] = v;
+        __syncthreads();
+        int t = 0;
+        for (int w = 0; w < W; ++w) t += sh.n[w];
+        return t;
+    }
+    MDP_DEV float block_max(float v) {
+        v = group_max<64>(v);
+        __syncthreads();
+        if (lane == 0) sh.f[wave] = v;
+        __syncthreads();
+        float t = sh.f[0];
+        for (int w = 1; w < W; ++w) t = larger(sh.f[w], t);
+        return t;
+    }
+    // sum over the threads up to and with this one; `all` over every thread
+    MDP_DEV double block_scan(double v, double& all) {
+        v = group_scan<64>(v);
+        __syncthreads();
+        if (lane == 63) sh.d[wave] = v;
+        __syncthreads();
+        double before = 0.0;
+        all = 0.0;
+        for (int w = 0; w < W; ++w) {
+            if (w < wave) before += sh.d[w];
+            all += sh.d[w];
+        }
+        return before + v;
+    }
+    MDP_DEV double exact_mass(const Settings& s) {
+        double t = 0.0;
+        each([&](int, const float (&v)[N]) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) t += s.weight(v[e], m);
+        });
+        return block_sum(t);
+    }
+
+    // A value not above the border, from the threads' largest entries, or -inf.  `mass`: the row's, in 32 bits.
+    MDP_DEV float bound_of(const Settings& s, float top, float mass) {
+        __syncthreads();
+        sh.maxima.top[tid] = top;
+        __syncthreads();
+        if (wave == 0) {
+            float v[W], w[W];
+            const float c = s.c32();
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                v[i] = sh.maxima.top[i * 64 + lane];
+                w[i] = __builtin_amdgcn_exp2f(larger((v[i] - m) * c, -300.0f));
+            }
+            const float aim = (float)s.p * mass * 1.0001f;             // above p S whatever 32 bits made of the sums
+            float bound = -kInf;
+            if (s.k > 0 || s.p < 1.0) {
+                const auto enough = [&](float from) {
+                    float q = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < W; ++i) q += v[i] >= from ? (s.k > 0 ? 1.0f : w[i]) : 0.0f;
+                    q = group_sum<64>(q);
+                    return s.k > 0 ? q >= (float)s.k : q >= aim;
+                };
+                float lo = (float)((double)m - 60.0 / s.c), hi = m;
+                if (enough(lo)) {
+                    // twelve halvings: 60 binary orders of magnitude down to 1/64 of one, a few entries more than needed
+                    for (int it = 0; it < 12; ++it) {
+                        const float mid = 0.5f * lo + 0.5f * hi;
+                        if (enough(mid)) lo = mid; else hi = mid;
+                    }
+                    bound = lo;
+                }
+            }
+            if (s.k == 0 && s.mp > 0.0) {
+                // lighter than min_p: never kept
+                const float light = (float)((double)m + log2(s.mp) / s.c);
+                bound = larger(light - 1e-3f * fabsf(light) - 1e-3f, bound);
+            }
+            if (lane == 0) sh.bound = bound;
+        }
+        __syncthreads();
+        return sh.bound;
+    }
+
+    // Gathers the entries >= bound in index order (position in the row beside each); their number, or -1 if there are too many.
+    MDP_DEV int gather(float bound) {
+        int mine = 0;
+        each([&](int, const float (&v)[N]) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) mine += v[e] >= bound;
+        });
+        mine = group_sum<64>(mine);
+        __syncthreads();
+        if (lane == 0) sh.n[wave] = mine;
+        __syncthreads();
+        int base = 0, total = 0;
+        for (int w = 0; w < W; ++w) {
+            if (w < wave) base += sh.n[w];
+            total += sh.n[w];
+        }
+        if (total > THREADS) return -1;
+        each([&](int step, const float (&v)[N]) {
+            int n = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) n += v[e] >= bound;
+            if (__any(n)) {
+                const int upto = group_scan<64>(n);
+                int to = base + upto - n;
+                const int i0 = (first + 64 * step + lane) * N - r.shift;
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (v[e] >= bound) {
+                        sh.list.x[to] = v[e] + 0.0f;
+                        sh.list.key[to] = (uint64_t)(~key_of(v[e])) << 32 | (uint32_t)(i0 + e);
+                        ++to;
+                    }
+                base += __shfl(upto, 63);
+            }
+        });
+        __syncthreads();
+        return total;
+    }
+
+    // sorts the threads' words, rising with the thread
+    MDP_DEV uint64_t sort(uint64_t v, int n) {
+        for (int size = 2; size < 2 * n; size <<= 1)
+            for (int stride = size >> 1; stride; stride >>= 1) {
+                uint64_t o;
+                if (stride < 64) o = __shfl_xor((unsigned long long)v, stride);
+                else {
+                    __syncthreads();
+                    sh.list.key[tid] = v;
+                    __syncthreads();
+                    o = sh.list.key[tid ^ stride];
+                }
+                const bool low = !(tid & stride), rising = !(tid & size);
+                v = (o < v) == (low == rising) ? o : v;
+            }
+        return v;
+    }
+
+    MDP_DEV void answer(const SampleArgs& g, int64_t row, int i, double w, double mass) {
+        g.actions[row] = i;
+        g.log_prob[row] = (float)log(w / mass);
+    }
+
+    // the draw among n gathered candidates, among which is everything that k, p and min_p keep
+    MDP_DEV void draw_from_list(const SampleArgs& g, int64_t row, const Settings& s, int n, double mass32) {
+        const bool in = tid < n;
+        const float x = in ? sh.list.x[tid] : 0.0f;
+        const uint64_t word = in ? sh.list.key[tid] : ~0ull;
+        const double w = in ? s.weight(x, m) : 0.0;
+        int padded = 64;
+        while (padded < n) padded <<= 1;
+        __syncthreads();
+        // sorted by (value falling, place rising): the low half of the word is the place in the row; the thread's place in the
+        // list is found again through it below
+        const uint64_t sorted = sort(word, padded);
+        const bool in_s = tid < n;
+        const double ws = in_s ? s.weight(of_key(~(uint32_t)(sorted >> 32)), m) : 0.0;
+        double all;
+        const double upto = block_scan(ws, all), before = upto - ws;
+        int kept = s.k > 0 ? min(s.k, n) : n;
+        if (s.p < 1.0) {
+            double held = mass32;
+            if (s.k > 0) held = block_sum(tid == kept - 1 ? upto : 0.0);
+            int short_of = block_sum((int)(tid < kept && before < s.p * held));
+            if (s.k == 0) {
+                // the row's mass in 32 bits decides unless the border is within its error (2^-17) of the aim
+                const int low = block_sum((int)(tid < kept && before < s.p * held * (1.0 - 7.7e-6)));
+                const int high = block_sum((int)(tid < kept && before < s.p * held * (1.0 + 7.7e-6)));
+                if (low != high) {
+                    held = exact_mass(s);
+                    short_of = block_sum((int)(tid < kept && before < s.p * held));
+                }
+            }
+            kept = min(kept, short_of);
+        }
+        kept = min(kept, block_sum((int)(in_s && ws >= s.mp)));
+        kept = max(kept, 1);
+        // the lowest word that is not kept tells by itself which entries of the list are
+        __syncthreads();
+        if (tid == kept - 1) sh.list.key[0] = sorted;
+        __syncthreads();
+        const uint64_t border = sh.list.key[0];
+        const double kw = in && word <= border ? w : 0.0;
+        double sum;
+        const double line = block_scan(kw, sum);
+        const double aim = s.u * sum;
+        if (tid == 0) { sh.found = THREADS; sh.last = 0; }
+        __syncthreads();
+        if (kw > 0.0) {
+            if (line > aim) atomicMin(&sh.found, tid);
+            atomicMax(&sh.last, tid);
+        }
+        __syncthreads();
+        const int who = sh.found < THREADS ? sh.found : sh.last;
+        if (tid == who) answer(g, row, (int)(uint32_t)word, kw, sum);
+    }
+
+    // the draw over the whole row
+    MDP_DEV void draw_from_row(const SampleArgs& g, int64_t row, const Settings& s) {
+        Border b{-__FLT_MAX__, 0x7fffffff, 0, 0.0, 0};
+        if (s.k > 0 || s.p < 1.0) {
+            const auto any = [](bool v) { return v; };
+            int allowed = 0;
+            each([&](int, const float (&v)[N]) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) allowed += v[e] > -kInf;
+            });
+            allowed = block_sum(allowed);
+            b = find_border(s, m, allowed, exact_mass(s),
+                [&](float from) {
+                    int n = 0;
+                    double q = 0.0;
+                    each([&](int, const float (&v)[N]) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) {
+                            const bool yes = v[e] >= from;
+                            n += yes;
+                            q += yes ? s.weight(v[e], m) : 0.0;
+                        }
+                    });
+                    const int count = block_sum(n);
+                    return Measure{count, block_sum(q)};
+                },
+                [&](float under) {
+                    float t = -kInf;
+                    each([&](int, const float (&v)[N]) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) t = v[e] < under ? larger(v[e], t) : t;
+                    });
+                    return block_max(t);
+                }, any);
+        }
+        const bool ranked = b.room < b.level;
+        int rank0 = 0;
+        if (ranked) {
+            int equal = 0;
+            each([&](int, const float (&v)[N]) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) equal += v[e] == b.tau;
+            });
+            equal = group_sum<64>(equal);
+            __syncthreads();
+            if (lane == 0) sh.n[wave] = equal;
+            __syncthreads();
+            for (int w = 0; w < wave; ++w) rank0 += sh.n[w];
+        }
+        // f(step, kept weights) in index order; false ends it
+        const auto kept_weights = [&](int step, const float (&v)[N], int& rank, double (&w)[N]) {
+            int mine = 0;
+            if (ranked) {
+                int equal = 0;
+#pragma unroll
+                for (int e = 0; e < N; ++e) equal += v[e] == b.tau;
+                const int upto = group_scan<64>(equal);
+                mine = rank + upto - equal;
+                rank += __shfl(upto, 63);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const bool equal = v[e] == b.tau;
+                const bool keep = v[e] > b.tau || (equal && (!ranked || mine < b.room));
+                mine += equal;
+                w[e] = keep ? s.weight(v[e], m) : 0.0;
+                w[e] = w[e] >= s.mp ? w[e] : 0.0;
+            }
+        };
+        double mass = 0.0;
+        int rank = rank0;
+        each([&](int step, const float (&v)[N]) {
+            double w[N];
+            kept_weights(step, v, rank, w);
+#pragma unroll
+            for (int e = 0; e < N; ++e) mass += w[e];
+        });
+        mass = group_sum<64>(mass);
+        __syncthreads();
+        if (lane == 0) sh.d[wave] = mass;
+        __syncthreads();
+        double total = 0.0, before = 0.0, run = 0.0;
+        for (int w = 0; w < W; ++w) total += sh.d[w];
+        const double aim = s.u * total;
+        int target = -1;
+        for (int w = 0; w < W; ++w) {
+            if (sh.d[w] > 0.0 && run <= aim) { target = w; before = run; }
+            run += sh.d[w];
+        }
+        if (wave != target) return;
+        rank = rank0;
+        bool open = true;
+        int found = -1;
+        double found_w = 1.0;
+        each([&](int step, const float (&v)[N]) {
+            if (!open) return;                                         // uniform over the wave
+            double w[N], own = 0.0;
+            kept_weights(step, v, rank, w);
+#pragma unroll
+            for (int e = 0; e < N; ++e) own += w[e];
+            const double upto = before + group_scan<64>(own);
+            const uint64_t over = __ballot(own > 0.0 && upto > aim), some = __ballot(own > 0.0);
+            if (some) {                                                // see the short rows
+                const int winner = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
+                double sum = upto - own, my_w = 1.0;
+                int my = -1;
+                bool looking = true;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    sum += w[e];
+                    if (looking && w[e] > 0.0) {
+                        my = (first + 64 * step + lane) * N - r.shift + e;
+                        my_w = w[e];
+                        looking = !(sum > aim);
+                    }
+                }
+                found = __shfl(my, winner);
+                found_w = __shfl(my_w, winner);
+            }
+            open = over == 0ull;
+            before = __shfl(upto, 63);
+        });
+        if (lane == 0) answer(g, row, found, found_w, total);
+    }
+};
+
+template <typename T, bool MASK, int THREADS, int H>
+__global__ __launch_bounds__(THREADS) void k_sample_long(SampleArgs g) {
+    using L = LongRow<T, MASK, THREADS, H>;
+    constexpr int N = Chunk<T>::N;
+    __shared__ typename L::Shared sh;
+    const int64_t row = blockIdx.x;
+    L q(g, row, sh);
+    const Settings s(g, row);
+    float top = -kInf;
+    q.each([&](int, const float (&v)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = larger(v[e], top);
+    });
+    q.m = q.block_max(top);
+    const bool empty = q.m == -kInf;
+    // the row's mass in 32 bits, and whether it has a distribution at all
+    float mass = 0.0f;
+    const float c = s.c32();
+    q.each([&](int, const float (&v)[N]) {
+        float part = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) part += __builtin_amdgcn_exp2f((v[e] - q.m) * c);
+        mass += part;
+    });
+    const double total = q.block_sum((double)mass);
+    if (empty || !(total > 0.0) || s.c != s.c) {
+        if (threadIdx.x == 0) {
+            g.actions[row] = -1;
+            g.log_prob[row] = empty && s.c == s.c ? 0.0f : __builtin_nanf("");
+        }
+        return;
+    }
+    if (!s.all()) {
+        const float bound = q.bound_of(s, top, (float)total);
+        if (bound > -kInf) {
+            const int n = q.gather(bound);
+            if (n > 0) {
+                q.draw_from_list(g, row, s, n, total);
+                return;
+            }
+        }
+    }
+    q.draw_from_row(g, row, s);
+}
+
+__global__ void k_state_advance(unsigned long long* state) { state[1] += 1ull; }
 
 // -- evaluation -------------------------------------------------------------------------------------------------------
 // One pass: about the largest entry m so far, s = sum w and t = sum w log2 w with w = 2^((x - m) log2(e) / T).  Entries that
@@ -652,31 +1142,6 @@ int check_rows(const char* what, const void* logits, int64_t rows, int64_t vocab
     return MDP_OK;
 }
 
-}  // namespace
-
-extern "C" int mdp_categorical_sample(const mdp_categorical_sample_t* a, void* stream) {
-    MDP_REQUIRE(a, "null arguments");
-    if (int rc = check_rows("categorical_sample", a->logits, a->rows, a->vocab, a->ld, a->dtype, a->mask, a->ld_mask)) return rc;
-    if (a->rows == 0) return MDP_OK;
-    MDP_REQUIRE(a->actions && a->log_prob, "categorical_sample: null output");
-    MDP_REQUIRE(a->u || a->state, "categorical_sample needs uniforms or a generator state {seed, epoch}");
-    SampleArgs g{a->logits, a->ld, a->mask, a->ld_mask, (int)a->vocab, a->temperature, a->top_k, a->top_p, a->min_p,
-                 a->temperature_scalar, a->top_k_scalar, a->top_p_scalar, a->min_p_scalar, a->u,
-                 (const unsigned long long*)a->state, a->actions, a->log_prob};
-    hipStream_t s = as_stream(stream);
-    const dim3 grid((unsigned)a->rows);
-    switch (a->dtype) {
-        case MDP_DTYPE_F32: hipLaunchKernelGGL((k_sample_row<float, 256>), grid, dim3(256), 0, s, g); break;
-        case MDP_DTYPE_BF16: hipLaunchKernelGGL((k_sample_row<bf16, 256>), grid, dim3(256), 0, s, g); break;
-        default: hipLaunchKernelGGL((k_sample_row<f16, 256>), grid, dim3(256), 0, s, g); break;
-    }
-    if (!a->u) hipLaunchKernelGGL(k_state_advance, dim3(1), dim3(1), 0, s, (unsigned long long*)a->state);
-    MDP_LAUNCH_CHECK();
-    return MDP_OK;
-}
-
-namespace {
-
 // The most chunks that a row can touch: one more than it fills where rows do not all start on a chunk's boundary.
 template <typename T>
 int most_chunks(const void* logits, int64_t ld, int64_t rows, int vocab) {
@@ -686,6 +1151,22 @@ int most_chunks(const void* logits, int64_t ld, int64_t rows, int vocab) {
 }
 
 // That number decides how many lanes hold a row; beyond 256 chunks (1024 floats, 2048 16-bit entries) a row is a block's.
+template <typename T, bool MASK>
+void launch_sample(const SampleArgs& g, hipStream_t s) {
+    const int chunks = most_chunks<T>(g.logits, g.ld, g.rows, g.vocab);
+    constexpr int K = 16 / Chunk<T>::N;                // 16 entries a lane
+#define SHORT(G)                                                                                                                \
+    if (chunks <= G * K) {                                                                                                      \
+        hipLaunchKernelGGL((k_sample_short<T, MASK, G, K>), dim3((unsigned)((g.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, s, g); \
+        return;                                                                                                                 \
+    }
+    SHORT(4) SHORT(8) SHORT(16) SHORT(32) SHORT(64)
+#undef SHORT
+    if (chunks <= 256 * 4) hipLaunchKernelGGL((k_sample_long<T, MASK, 256, 4>), dim3((unsigned)g.rows), dim3(256), 0, s, g);
+    else if (chunks <= 1024 * 4) hipLaunchKernelGGL((k_sample_long<T, MASK, 1024, 4>), dim3((unsigned)g.rows), dim3(1024), 0, s, g);
+    else hipLaunchKernelGGL((k_sample_long<T, MASK, 1024, 16>), dim3((unsigned)g.rows), dim3(1024), 0, s, g);
+}
+
 template <typename T, bool MASK>
 void launch_evaluate(const EvalArgs& g, hipStream_t s) {
     const int chunks = most_chunks<T>(g.logits, g.ld, g.rows, g.vocab);
@@ -722,6 +1203,22 @@ void by_type(int dtype, bool mask, F&& f) {
 }
 
 }  // namespace
+
+extern "C" int mdp_categorical_sample(const mdp_categorical_sample_t* a, void* stream) {
+    MDP_REQUIRE(a, "null arguments");
+    if (int rc = check_rows("categorical_sample", a->logits, a->rows, a->vocab, a->ld, a->dtype, a->mask, a->ld_mask)) return rc;
+    if (a->rows == 0) return MDP_OK;
+    MDP_REQUIRE(a->actions && a->log_prob, "categorical_sample: null output");
+    MDP_REQUIRE(a->u || a->state, "categorical_sample needs uniforms or a generator state {seed, epoch}");
+    SampleArgs g{a->logits, a->ld, a->mask, a->ld_mask, (int)a->vocab, a->rows, a->temperature, a->top_k, a->top_p, a->min_p,
+                 a->temperature_scalar, a->top_k_scalar, a->top_p_scalar, a->min_p_scalar, a->u,
+                 (const unsigned long long*)a->state, a->actions, a->log_prob};
+    hipStream_t s = as_stream(stream);
+    by_type(a->dtype, a->mask, [&](auto t, auto m) { launch_sample<decltype(t), decltype(m)::value>(g, s); });
+    if (!a->u) hipLaunchKernelGGL(k_state_advance, dim3(1), dim3(1), 0, s, (unsigned long long*)a->state);
+    MDP_LAUNCH_CHECK();
+    return MDP_OK;
+}
 
 extern "C" int mdp_categorical_evaluate(const mdp_categorical_eval_t* a, void* stream) {
     MDP_REQUIRE(a, "null arguments");

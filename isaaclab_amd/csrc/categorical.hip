@@ -27,22 +27,20 @@ MDP_DEV uint32_t key_of(float x) {
 }
 MDP_DEV float of_key(uint32_t k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
 
-// 2^t for t <= 0 in 64 bits: t = n + f with |f| <= 1/2, 2^f by its Taylor series (ln 2)^k / k! f^k; the first term left
-// out, (ln 2 / 2)^13 / 13!, is 1.7e-16.  64-bit multiply-adds issue at the rate of 32-bit ones on this chip.
+// 2^t for t <= 0 in 64 bits: t = n + f with |f| <= 1/2, and (2^f - 1) / f by the polynomial through its values at nine Chebyshev
+// points of [-1/2, 1/2]; at most 3.7e-14 of the result off, and 1 at 0.  64-bit multiply-adds issue at the rate of 32-bit ones on
+// this chip.  0 for -inf; a NaN is the caller's to look for.
 MDP_DEV double exp2_neg(double t) {
-    t = t < -1100.0 ? -1100.0 : t;               // below the smallest denormal: 0
+    t = __builtin_fmax(t, -1100.0);                    // below the smallest denormal: 0
     const double n = __builtin_rint(t), f = t - n;
-    double p = 2.5678435993488196e-11;
-    p = fma(p, f, 4.44553827187081e-10);
-    p = fma(p, f, 7.054911620801121e-09);
-    p = fma(p, f, 1.0178086009239696e-07);
-    p = fma(p, f, 1.3215486790144305e-06);
-    p = fma(p, f, 1.5252733804059838e-05);
-    p = fma(p, f, 0.00015403530393381606);
-    p = fma(p, f, 0.0013333558146428441);
-    p = fma(p, f, 0.009618129107628477);
-    p = fma(p, f, 0.055504108664821576);
-    p = fma(p, f, 0.2402265069591007);
+    double p = 1.0203121113055101e-07;
+    p = fma(p, f, 1.3255224878933224e-06);
+    p = fma(p, f, 1.5252686846120593e-05);
+    p = fma(p, f, 0.00015403455852451632);
+    p = fma(p, f, 0.0013333558179043103);
+    p = fma(p, f, 0.009618129159402562);
+    p = fma(p, f, 0.055504108664760424);
+    p = fma(p, f, 0.2402265069581299);
     p = fma(p, f, 0.6931471805599453);
     p = fma(p, f, 1.0);
     return __builtin_ldexp(p, (int)n);
@@ -107,49 +105,83 @@ struct Row {
 // the larger of two numbers, b where a is a NaN (one instruction, without fmaxf's canonicalisation of its operands)
 MDP_DEV float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, kInf); }
 
-// lane i gets lane i ^ m's value (m < 4), or, for m = 4 and 8, that of the lane mirrored inside 8 or 16: what a reduction
-// needs whose groups of m already agree
+// lane i gets lane i ^ M's value (M < 4), for M = 4 and 8 that of the lane mirrored inside 8 or 16, for M = 16 and 32 that of a
+// lane in the other half of 32 or 64: what a reduction needs whose groups of M already agree
 template <int M>
-MDP_DEV float across(float v) {
-    const int x = __float_as_int(v);
-    if constexpr (M == 1) return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0xB1, 0xf, 0xf, true));        // quad_perm 1 0 3 2
-    else if constexpr (M == 2) return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0x4E, 0xf, 0xf, true));   // quad_perm 2 3 0 1
-    else if constexpr (M == 4) return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, true));  // row_half_mirror
-    else if constexpr (M == 8) return __int_as_float(__builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, true));  // row_mirror
-    else return __shfl_xor(v, M);
+MDP_DEV uint32_t across_word(uint32_t x) {
+    if constexpr (M == 1) return __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
+    else if constexpr (M == 2) return __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+    else if constexpr (M == 4) return __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, true);  // row_half_mirror
+    else return __builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, true);                        // row_mirror
 }
-template <int G, class F>
-MDP_DEV float over_group(float v, F&& f) {             // every lane of a group of G gets the result
-    if constexpr (G > 1) v = f(v, across<1>(v));
-    if constexpr (G > 2) v = f(v, across<2>(v));
-    if constexpr (G > 4) v = f(v, across<4>(v));
-    if constexpr (G > 8) v = f(v, across<8>(v));
-    if constexpr (G > 16) v = f(v, across<16>(v));
-    if constexpr (G > 32) v = f(v, across<32>(v));
+// both halves' values, the same for all lanes of a pair of rows of M lanes
+template <int M>
+MDP_DEV void halves(uint32_t x, uint32_t& a, uint32_t& b) {
+    if constexpr (M == 16) { const auto q = __builtin_amdgcn_permlane16_swap(x, x, false, false); a = q[0]; b = q[1]; }
+    else { const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false); a = q[0]; b = q[1]; }
+}
+template <int M, typename V, class F>
+MDP_DEV V over_step(V v, F&& f) {
+    constexpr int L = sizeof(V) / 4;
+    struct Words { uint32_t w[L]; } x = __builtin_bit_cast(Words, v), y;
+    if constexpr (M < 16) {
+#pragma unroll
+        for (int i = 0; i < L; ++i) y.w[i] = across_word<M>(x.w[i]);
+        return f(v, __builtin_bit_cast(V, y));
+    } else {
+#pragma unroll
+        for (int i = 0; i < L; ++i) halves<M>(x.w[i], x.w[i], y.w[i]);
+        return f(__builtin_bit_cast(V, x), __builtin_bit_cast(V, y));
+    }
+}
+template <int G, typename V, class F>
+MDP_DEV V over_group(V v, F&& f) {                     // every lane of a group of G gets the result
+    if constexpr (G > 1) v = over_step<1>(v, f);
+    if constexpr (G > 2) v = over_step<2>(v, f);
+    if constexpr (G > 4) v = over_step<4>(v, f);
+    if constexpr (G > 8) v = over_step<8>(v, f);
+    if constexpr (G > 16) v = over_step<16>(v, f);
+    if constexpr (G > 32) v = over_step<32>(v, f);
     return v;
 }
 template <int G>
 MDP_DEV float group_max(float v) { return over_group<G>(v, [](float a, float b) { return larger(a, b); }); }
-template <int G>
-MDP_DEV float group_sum(float v) { return over_group<G>(v, [](float a, float b) { return a + b; }); }
+template <int G, typename V>
+MDP_DEV V group_sum(V v) { return over_group<G>(v, [](V a, V b) { return a + b; }); }
 
-template <int G>
-MDP_DEV double group_sum(double v) {
-    for (int o = 1; o < G; o <<= 1) v += __shfl_xor(v, o);
-    return v;
+// the value O lanes below in a row of 16, 0 where there is none
+template <int O, typename V>
+MDP_DEV V from_below(V v) {
+    constexpr int L = sizeof(V) / 4;
+    struct Words { uint32_t w[L]; } x = __builtin_bit_cast(Words, v);
+#pragma unroll
+    for (int i = 0; i < L; ++i) x.w[i] = __builtin_amdgcn_update_dpp(0, x.w[i], 0x110 + O, 0xf, 0xf, false);     // row_shr
+    return __builtin_bit_cast(V, x);
 }
-template <int G>
-MDP_DEV int group_sum(int v) {
-    for (int o = 1; o < G; o <<= 1) v += __shfl_xor(v, o);
-    return v;
+template <typename V>
+MDP_DEV V of_lane(V v, int lane) {                     // uniform lane
+    constexpr int L = sizeof(V) / 4;
+    struct Words { uint32_t w[L]; } x = __builtin_bit_cast(Words, v);
+#pragma unroll
+    for (int i = 0; i < L; ++i) x.w[i] = __builtin_amdgcn_readlane(x.w[i], lane);
+    return __builtin_bit_cast(V, x);
 }
 // sum over the lanes of the group up to and with this one
 template <int G, typename V>
 MDP_DEV V group_scan(V v) {
-    const int lane = threadIdx.x % G;
-    for (int o = 1; o < G; o <<= 1) {
-        const V up = __shfl_up(v, o);
-        if (lane >= o) v += up;
+    const int at = threadIdx.x & 63, lane = at % G;
+    V up = from_below<1>(v);
+    v += lane >= 1 ? up : V(0);
+    up = from_below<2>(v);
+    if constexpr (G > 2) v += lane >= 2 ? up : V(0);
+    up = from_below<4>(v);
+    if constexpr (G > 4) v += lane >= 4 ? up : V(0);
+    up = from_below<8>(v);
+    if constexpr (G > 8) v += lane >= 8 ? up : V(0);
+    if constexpr (G == 32) v += lane >= 16 ? (at >= 32 ? of_lane(v, 47) : of_lane(v, 15)) : V(0);
+    if constexpr (G == 64) {
+        const V a = of_lane(v, 15), b = of_lane(v, 31), c = of_lane(v, 47);
+        v += at < 16 ? V(0) : at < 32 ? a : at < 48 ? a + b : a + b + c;
     }
     return v;
 }
@@ -237,8 +269,7 @@ MDP_DEV Border find_border(const Settings& s, float m, int allowed, double total
     if (any(by_k)) {
         Border q = search(m, s.c, allowed, measure, below, [&](Measure x) { return x.count >= s.k; }, [&](bool busy) { return any(by_k && busy); });
         if (by_k) {
-            b = q;
-            b.room = s.k - q.count;
+            b.tau = q.tau; b.level = q.level; b.room = s.k - q.count;
             held = q.above + (double)b.room * s.weight(q.tau, m);
         }
     }
@@ -250,8 +281,12 @@ MDP_DEV Border find_border(const Settings& s, float m, int allowed, double total
             // of the level those that have less than the aim before them, one at least
             const double need = (aim - q.above) / s.weight(q.tau, m);
             q.room = need < 1.0 ? 1 : need < (double)q.level ? (int)__builtin_ceil(need) : q.level;
-            if (by_k && !(q.tau > b.tau)) { q = b.room < q.room || q.tau < b.tau ? b : q; }
-            b = q;
+            // of two borders the higher; at one value the smaller room
+            if (!by_k || q.tau > b.tau) {
+                b.tau = q.tau; b.level = q.level; b.room = q.room;
+            } else if (q.tau == b.tau) {
+                b.room = min(b.room, q.room);
+            }
         }
     }
     return b;
@@ -272,14 +307,16 @@ __global__ __launch_bounds__(256) void k_sample_short(SampleArgs g) {
     for (int k = 0; k < K; ++k) r.template load<MASK>(k * G + lane, x[k]);
     const Settings s(g, row);
     float m = -kInf;
+    bool broken = false;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            x[k][e] += 0.0f;                                           // one zero
+            broken |= !(x[k][e] < kInf);
             m = larger(x[k][e], m);
         }
     m = group_max<G>(m);
+    broken = (__ballot(broken) & group) != 0 || s.c != s.c;
     const bool empty = m == -kInf;
     double w[K][N], total = 0.0;
 #pragma unroll
@@ -290,7 +327,7 @@ __global__ __launch_bounds__(256) void k_sample_short(SampleArgs g) {
             total += w[k][e];
         }
     total = group_sum<G>(total);
-    const bool good = total > 0.0 && !empty;                           // false for a NaN too
+    const bool good = !broken && !empty;
     const auto any = [&](bool v) { return __any(v && good) != 0; };
     if (any(!s.all())) {
         int allowed = 0;
@@ -388,7 +425,7 @@ __global__ __launch_bounds__(256) void k_sample_short(SampleArgs g) {
         }
     }
     g.actions[mine] = good ? found : -1;
-    g.log_prob[mine] = good ? (float)log(found_w / mass) : empty && s.c == s.c ? 0.0f : __builtin_nanf("");
+    g.log_prob[mine] = good ? (float)log(found_w / mass) : broken ? __builtin_nanf("") : 0.0f;
 }
 
 // Longer rows: a block a row.  Each wave owns a contiguous piece of the row, so that running sums follow the index; of it every
@@ -455,6 +492,18 @@ struct LongRow {
             f(h, v);
         }
     }
+    // the same with every chunk read again: for what is asked of a whole row only where the candidates do not decide.  A loop, where
+    // the registers would need the code once for each chunk that they hold.
+    template <class F>
+    MDP_DEV void each_again(F&& f) const {
+        for (int h = 0; h < steps; ++h) {
+            const Chunk<T> q = chunk(h);
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = q.at(e);
+            f(h, v);
+        }
+    }
     MDP_DEV double block_sum(double v) {
         v = group_sum<64>(v);
         __syncthreads();
@@ -498,7 +547,7 @@ struct LongRow {
     }
     MDP_DEV double exact_mass(const Settings& s) {
         double t = 0.0;
-        each([&](int, const float (&v)[N]) {
+        each_again([&](int, const float (&v)[N]) {
 #pragma unroll
             for (int e = 0; e < N; ++e) t += s.weight(v[e], m);
         });
@@ -671,7 +720,7 @@ struct LongRow {
         if (s.k > 0 || s.p < 1.0) {
             const auto any = [](bool v) { return v; };
             int allowed = 0;
-            each([&](int, const float (&v)[N]) {
+            each_again([&](int, const float (&v)[N]) {
 #pragma unroll
                 for (int e = 0; e < N; ++e) allowed += v[e] > -kInf;
             });
@@ -680,7 +729,7 @@ struct LongRow {
                 [&](float from) {
                     int n = 0;
                     double q = 0.0;
-                    each([&](int, const float (&v)[N]) {
+                    each_again([&](int, const float (&v)[N]) {
 #pragma unroll
                         for (int e = 0; e < N; ++e) {
                             const bool yes = v[e] >= from;
@@ -693,7 +742,7 @@ struct LongRow {
                 },
                 [&](float under) {
                     float t = -kInf;
-                    each([&](int, const float (&v)[N]) {
+                    each_again([&](int, const float (&v)[N]) {
 #pragma unroll
                         for (int e = 0; e < N; ++e) t = v[e] < under ? larger(v[e], t) : t;
                     });
@@ -704,7 +753,7 @@ struct LongRow {
         int rank0 = 0;
         if (ranked) {
             int equal = 0;
-            each([&](int, const float (&v)[N]) {
+            each_again([&](int, const float (&v)[N]) {
 #pragma unroll
                 for (int e = 0; e < N; ++e) equal += v[e] == b.tau;
             });
@@ -736,7 +785,7 @@ struct LongRow {
         };
         double mass = 0.0;
         int rank = rank0;
-        each([&](int step, const float (&v)[N]) {
+        each_again([&](int step, const float (&v)[N]) {
             double w[N];
             kept_weights(step, v, rank, w);
 #pragma unroll
@@ -759,7 +808,7 @@ struct LongRow {
         bool open = true;
         int found = -1;
         double found_w = 1.0;
-        each([&](int step, const float (&v)[N]) {
+        each_again([&](int step, const float (&v)[N]) {
             if (!open) return;                                         // uniform over the wave
             double w[N], own = 0.0;
             kept_weights(step, v, rank, w);

@@ -226,85 +226,262 @@ struct Settings {
     MDP_DEV double weight(float x, float m) const { return exp2_neg(((double)x - (double)m) * c); }
 };
 
-// Border of what is kept: entries above tau, and the first `room` of the `level` entries equal to it.
+// What is kept is a prefix of the row sorted by (value falling, place rising): everything up to and with one entry.
 struct Border {
     float tau;
-    int room, level;
-    double above;                                      // mass above tau
-    int count;                                         // entries above tau
+    int place;
+    MDP_DEV bool keeps(float x, int i) const { return x > tau || (x == tau && i <= place); }
 };
+MDP_DEV Border everything() { return Border{-__FLT_MAX__, 0x7fffffff}; }
 
-MDP_DEV float next_above(float x) { return of_key(key_of(x) + 1u); }
+// Nothing that is computed from x before is kept for after this: sixteen entries' worth of it would not fit the registers
+template <typename V>
+MDP_DEV void anew(V& x) { asm volatile("" : "+v"(x)); }
 
-// The largest entry tau with reaches(count, mass) of the entries >= tau, which has to hold for the lowest entry and grow with
-// count and mass.  measure(P) = {count, mass} of the entries >= P, the same for all who search together; below(P) = the largest
-// entry < P.  [lo, hi) always holds the answer: halved by value -- first about where the weights end -- and by key once values
-// stop narrowing it, until one entry or one value is left in it.
-struct Measure { int count; double mass; };
-template <class M, class B, class R, class Any>
-MDP_DEV Border search(float m, double c, int allowed, M&& measure, B&& below, R&& reaches, Any&& any) {
-    float lo = -__FLT_MAX__, hi = next_above(m);
-    Measure at_lo{allowed, 0.0}, at_hi{0, 0.0};
-    const float first = (float)((double)m - 60.0 / c);
-    for (int it = 0;; ++it) {
-        const bool busy = at_lo.count - at_hi.count > 1 && next_above(lo) < hi;
-        if (!any(busy)) break;
-        float mid = it == 0 ? first : 0.5f * lo + 0.5f * hi;
-        if (it > 24 || !(mid > lo && mid < hi)) mid = of_key(key_of(lo) + (key_of(hi) - key_of(lo)) / 2u);
-        const Measure q = measure(mid);
-        if (busy) {
-            if (reaches(q)) { lo = mid; at_lo = q; }
-            else { hi = mid; at_hi = q; }
+// Finds the last entry of the shortest prefix that holds `aim`, counting entries (COUNT) or their weights.  C is what searches a row
+// together -- a group of lanes or a block -- and gives
+//   each(f): f(x, place, w) for each of this lane's entries, w() its weight; weight(x); sum, highest, lowest over all; scan: the sum
+//   over the lanes up to and with this one; sync; any: over the lanes that run this loop in step; size, rank: lanes and this lane's
+//   number; hist[buckets] in shared memory, and there a list of up to `capacity` entries: gather<COUNT>(p) fills it with those that p
+//   names, last_kept<COUNT>(n, above, aim) finds the border among its n, with `above` before them; nth_equal(x, r): the place of the
+//   r-th entry equal to x (r from 1).
+// Entries are counted into buckets that fall with the value: about the maximum first, a bucket a small part of a binary order of
+// magnitude (entries below 24 of them share the last).  The bucket in which the aim is reached, by 32-bit fixed point, is confirmed
+// in 64 bits; its few entries are then looked at one by one.  If they are too many, the bucket is cut again, by keys, which ends
+// with one value.
+template <bool COUNT, class C>
+MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double total, bool active) {
+    Border border = everything();
+    float per = (float)C::buckets / 24.0f * s.c32();              // buckets for a difference of 1
+    double scale = COUNT ? 1.0 : 2147483648.0 / total;                 // all weights together: half of what 32 bits hold
+    float top = m, bottom = -__FLT_MAX__;
+    double above = 0.0;
+    int shift = -1;                                    // by value; later by key >> shift
+    const auto bucket = [&](float x) {
+        if (c.any(shift >= 0)) {
+            float again = x;
+            anew(again);
+            if (shift >= 0) return (int)((key_of(top) - key_of(again)) >> shift);
         }
+        return (int)(uint32_t)fminf((top - x) * per, (float)(C::buckets - 1));
+    };
+    while (c.any(active)) {
+        c.sync();
+        for (int i = c.rank; i < C::buckets; i += C::size) c.hist[i] = 0u;
+        c.sync();
+        anew(per);
+        anew(scale);
+        c.each([&](float x, int, auto&& w) {
+            if (active && x <= top && x >= bottom) atomicAdd(&c.hist[bucket(x)], COUNT ? 1u : (uint32_t)fma(w(), scale, 0.5));
+        });
+        c.sync();
+        constexpr int PER = C::buckets / C::size;
+        const double need = (aim - above) * scale;
+        double mine = 0.0;
+        uint32_t q[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            q[i] = c.hist[c.rank * PER + i];
+            mine += (double)q[i];
+        }
+        double run = c.scan(mine) - mine;
+        int b = C::buckets;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            run += (double)q[i];
+            if (b == C::buckets && run >= need && q[i]) b = c.rank * PER + i;
+        }
+        b = (int)c.lowest((float)b);
+        if (b == C::buckets) b = C::buckets - 1;
+        // confirm
+        int count;
+        double more;
+        bool sure = false;
+        do {
+            count = 0;
+            more = 0.0;
+            double in = 0.0;
+            anew(per);
+            c.each([&](float x, int, auto&& w) {
+                const int at = x <= top && x >= bottom ? bucket(x) : C::buckets;
+                const double v = COUNT ? 1.0 : w();
+                more += at < b ? v : 0.0;
+                in += at == b ? v : 0.0;
+                count += at == b;
+            });
+            count = c.sum(count);
+            more = c.sum(more);
+            in = c.sum(in);
+            int to = b;
+            if (above + more >= aim && b > 0) to = b - 1;
+            else if (above + more + in < aim && b < C::buckets - 1) to = b + 1;
+            else sure = true;
+            b = to;
+        } while (c.any(active && !sure));
+        const bool few = count <= C::capacity;
+        anew(per);
+        if (c.any(active && few)) {
+            c.template gather<COUNT>([&](float x) { return active && few && x <= top && x >= bottom && bucket(x) == b; });
+            const Border found = c.template last_kept<COUNT>(active && few ? count : 0, above + more, aim);
+            if (active && few) border = found;
+        }
+        if (c.any(active && !few)) {
+            float hi = -kInf, lo = kInf;
+            anew(per);
+            c.each([&](float x, int, auto&&) {
+                if (x <= top && x >= bottom && bucket(x) == b) { hi = fmaxf(hi, x); lo = fminf(lo, x); }
+            });
+            hi = c.highest(hi);
+            lo = c.lowest(lo);
+            const bool one = hi == lo;
+            if (c.any(active && !few && one)) {
+                const double v = COUNT ? 1.0 : c.weight(hi), want = (aim - (above + more)) / v;
+                const int r = want < 1.0 ? 1 : want < (double)count ? (int)__builtin_ceil(want) : count;
+                const int place = c.nth_equal(hi, r);
+                if (active && !few && one) border = Border{hi, place};
+            }
+            if (!few && !one) {
+                top = hi;
+                bottom = lo;
+                above += more;
+                const uint32_t range = key_of(hi) - key_of(lo);
+                shift = 0;
+                while (range >> shift >= (uint32_t)C::buckets) ++shift;
+            }
+            active = active && !few && !one;
+        } else active = false;
     }
-    return Border{below(hi), 0, at_lo.count - at_hi.count, at_hi.mass, at_hi.count};
+    return border;
 }
 
-// The border that k and p draw together.
-template <class M, class B, class Any>
-MDP_DEV Border find_border(const Settings& s, float m, int allowed, double total, M&& measure, B&& below, Any&& any) {
-    Border b{-__FLT_MAX__, 0x7fffffff, 0, 0.0, 0};
-    const bool by_k = s.k > 0 && s.k < allowed;
-    double held = total;                               // mass of the first k
-    if (any(by_k)) {
-        Border q = search(m, s.c, allowed, measure, below, [&](Measure x) { return x.count >= s.k; }, [&](bool busy) { return any(by_k && busy); });
-        if (by_k) {
-            b.tau = q.tau; b.level = q.level; b.room = s.k - q.count;
-            held = q.above + (double)b.room * s.weight(q.tau, m);
+// The border that k and p draw together, of `allowed` entries that weigh `total`.
+template <class C>
+MDP_DEV Border border_of(C& c, const Settings& s, float m, double total, int allowed) {
+    Border b = everything();
+    const bool by_k = s.k > 0 && s.k < allowed, by_p = s.p < 1.0;
+    double held = total;
+    if (c.any(by_k)) {
+        const Border f = find_border<true>(c, s, m, (double)s.k, 1.0, by_k);
+        if (by_k) b = f;
+        if (c.any(by_k && by_p)) {
+            double kept = 0.0;
+            c.each([&](float x, int i, auto&& w) { kept += b.keeps(x, i) ? w() : 0.0; });
+            held = c.sum(kept);
         }
     }
-    const bool by_p = s.p < 1.0;
-    if (any(by_p)) {
-        const double aim = s.p * held;
-        Border q = search(m, s.c, allowed, measure, below, [&](Measure x) { return x.mass >= aim; }, [&](bool busy) { return any(by_p && busy); });
-        if (by_p) {
-            // of the level those that have less than the aim before them, one at least
-            const double need = (aim - q.above) / s.weight(q.tau, m);
-            q.room = need < 1.0 ? 1 : need < (double)q.level ? (int)__builtin_ceil(need) : q.level;
-            // of two borders the higher; at one value the smaller room
-            if (!by_k || q.tau > b.tau) {
-                b.tau = q.tau; b.level = q.level; b.room = q.room;
-            } else if (q.tau == b.tau) {
-                b.room = min(b.room, q.room);
-            }
-        }
+    if (c.any(by_p)) {
+        const Border f = find_border<false>(c, s, m, s.p * held, total, by_p);
+        if (by_p && (f.tau > b.tau || (f.tau == b.tau && f.place < b.place))) b = f;
     }
     return b;
 }
 
-// Rows of up to G K chunks, 16 entries a lane: G lanes of a wave hold a row and its weights in registers.  A question about the row
-// is a sum over 16 registers and one over G lanes.  Groups of a wave go through their loops together until the last is done.
+// Shared memory that lanes of one wave pass to each other: no barrier, only the order of its accesses
+MDP_DEV void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Rows of up to G K chunks, 16 entries a lane: G lanes of a wave hold a row and its weights in registers.  Groups of a wave go
+// through their loops together until the last is done.
+template <typename T, int G, int K>
+struct ShortRow {
+    static constexpr int N = Chunk<T>::N, size = G, buckets = 4 * G, capacity = G;
+    struct Shared { uint32_t hist[buckets]; float x[G]; int place[G]; double value[G]; };
+    float x[K][N];
+    double w[K][N];
+    int rank, shift;                                   // this lane's number; the row's shift
+    uint32_t* hist;
+    Shared* sh;
+    bool good;
+    float m;
+    const Settings* s;
+
+    MDP_DEV int place(int k, int e) const { return (k * G + rank) * N - shift + e; }
+    template <class F>
+    MDP_DEV void each(F&& f) const {
+        int base = rank * N - shift;
+        anew(base);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < N; ++e) f(x[k][e], base + k * G * N + e, [&] { return w[k][e]; });
+    }
+    MDP_DEV double weight(float v) const { return s->weight(v, m); }
+    template <typename V> MDP_DEV V sum(V v) const { return group_sum<G>(v); }
+    MDP_DEV float highest(float v) const { return group_max<G>(v); }
+    MDP_DEV float lowest(float v) const { return -group_max<G>(-v); }
+    template <typename V> MDP_DEV V scan(V v) const { return group_scan<G>(v); }
+    MDP_DEV void sync() const { wave_sync(); }
+    MDP_DEV bool any(bool v) const { return __any(v && good) != 0; }
+    template <bool COUNT, class P>
+    MDP_DEV void gather(P&& p) const {
+        int n = 0;
+        each([&](float v, int, auto&&) { n += p(v); });
+        int to = scan(n) - n;
+        if (n)
+            each([&](float v, int i, auto&& w) {
+                if (p(v)) {
+                    sh->x[to] = v;
+                    sh->place[to] = i;
+                    sh->value[to] = COUNT ? 1.0 : w();
+                    ++to;
+                }
+            });
+        sync();
+    }
+    template <bool COUNT>
+    MDP_DEV Border last_kept(int n, double above, double aim) const {
+        const bool in = rank < n;
+        const float v = in ? sh->x[rank] : 0.0f;
+        const int i = in ? sh->place[rank] : 0;
+        double before = above;
+        int order = 0;
+        for (int j = 0; __any(j < n); ++j) {
+            const float o = sh->x[j];                  // beyond n: of no effect
+            const bool first = j < n && (o > v || (o == v && sh->place[j] < i));
+            before += first ? sh->value[j] : 0.0;
+            order += first;
+        }
+        int kept = sum((int)(in && before < aim));
+        kept = kept ? kept : 1;
+        const bool me = in && order == kept - 1;
+        return Border{highest(me ? v : -kInf), sum(me ? i : 0)};
+    }
+    MDP_DEV int nth_equal(float v, int r) const {
+        int seen = 0, at = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            int equal = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) equal += x[k][e] == v;
+            const int upto = scan(equal);
+            int rank_of = seen + upto - equal;
+            seen += sum(equal);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                rank_of += x[k][e] == v;
+                if (x[k][e] == v && rank_of == r) at = place(k, e);
+            }
+        }
+        return sum(at);
+    }
+};
+
 template <typename T, bool MASK, int G, int K>
-__global__ __launch_bounds__(256) void k_sample_short(SampleArgs g) {
+__global__ __launch_bounds__(256, 4) void k_sample_short(SampleArgs g) {
+    using R = ShortRow<T, G, K>;
     constexpr int N = Chunk<T>::N;
+    __shared__ typename R::Shared shared[256 / G];
     const int64_t mine = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
     const int64_t row = mine < g.rows ? mine : g.rows - 1;             // lanes without a row of their own repeat the last
     const int lane = threadIdx.x % G, at = threadIdx.x & 63;
     const uint64_t group = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1ull)) << (at - lane);
     const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
-    float x[K][N];
+    R q;
 #pragma unroll
-    for (int k = 0; k < K; ++k) r.template load<MASK>(k * G + lane, x[k]);
+    for (int k = 0; k < K; ++k) r.template load<MASK>(k * G + lane, q.x[k]);
     const Settings s(g, row);
     float m = -kInf;
     bool broken = false;
@@ -312,72 +489,41 @@ __global__ __launch_bounds__(256) void k_sample_short(SampleArgs g) {
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            broken |= !(x[k][e] < kInf);
-            m = larger(x[k][e], m);
+            broken |= !(q.x[k][e] < kInf);
+            m = larger(q.x[k][e], m);
         }
     m = group_max<G>(m);
     broken = (__ballot(broken) & group) != 0 || s.c != s.c;
     const bool empty = m == -kInf;
-    double w[K][N], total = 0.0;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            w[k][e] = s.weight(x[k][e], empty ? 0.0f : m);
-            total += w[k][e];
-        }
-    total = group_sum<G>(total);
-    const bool good = !broken && !empty;
-    const auto any = [&](bool v) { return __any(v && good) != 0; };
-    if (any(!s.all())) {
+        for (int e = 0; e < N; ++e) q.w[k][e] = s.weight(q.x[k][e], empty ? 0.0f : m);
+    q.rank = lane;
+    q.shift = r.shift;
+    q.sh = &shared[threadIdx.x / G];
+    q.hist = q.sh->hist;
+    q.good = !broken && !empty;
+    q.m = m;
+    q.s = &s;
+    if (q.any(!s.all())) {
+        double total = 0.0;
         int allowed = 0;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int e = 0; e < N; ++e) allowed += x[k][e] > -kInf;
-        allowed = group_sum<G>(allowed);
-        const Border b = find_border(s, m, allowed, total,
-            [&](float from) {
-                Measure q{0, 0.0};
-#pragma unroll
-                for (int k = 0; k < K; ++k)
-#pragma unroll
-                    for (int e = 0; e < N; ++e) {
-                        const bool in = x[k][e] >= from;
-                        q.count += in;
-                        q.mass += in ? w[k][e] : 0.0;
-                    }
-                return Measure{group_sum<G>(q.count), group_sum<G>(q.mass)};
-            },
-            [&](float under) {
-                float v = -kInf;
-#pragma unroll
-                for (int k = 0; k < K; ++k)
-#pragma unroll
-                    for (int e = 0; e < N; ++e) v = x[k][e] < under ? larger(x[k][e], v) : v;
-                return group_max<G>(v);
-            }, any);
-        const bool ranked = b.room < b.level;                          // only some of the level stay, by lowest index
-        int rank0 = 0;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            int rank = rank0;
-            if (any(ranked)) {
-                int equal = 0;
-#pragma unroll
-                for (int e = 0; e < N; ++e) equal += x[k][e] == b.tau;
-                const int upto = group_scan<G>(equal);
-                rank = rank0 + upto - equal;
-                rank0 += __shfl(upto, at - lane + G - 1);
-            }
-#pragma unroll
             for (int e = 0; e < N; ++e) {
-                const bool equal = x[k][e] == b.tau;
-                const bool keep = (x[k][e] > b.tau || (equal && (!ranked || rank < b.room))) && w[k][e] >= s.mp;
-                rank += equal;
-                w[k][e] = keep ? w[k][e] : 0.0;
+                total += q.w[k][e];
+                allowed += q.x[k][e] > -kInf;
             }
-        }
+        total = group_sum<G>(total);
+        allowed = group_sum<G>(allowed);
+        const Border b = border_of(q, s, m, total, allowed);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                q.w[k][e] = b.keeps(q.x[k][e], q.place(k, e)) && q.w[k][e] >= s.mp ? q.w[k][e] : 0.0;
     }
     // masses by chunk index; the chunk row k that holds the aim, the lane in it, the entry in that
     double part[K], mass = 0.0, sums[K];
@@ -385,7 +531,7 @@ __global__ __launch_bounds__(256) void k_sample_short(SampleArgs g) {
     for (int k = 0; k < K; ++k) {
         part[k] = 0.0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) part[k] += w[k][e];
+        for (int e = 0; e < N; ++e) part[k] += q.w[k][e];
         sums[k] = group_sum<G>(part[k]);
         mass += sums[k];
     }
@@ -405,7 +551,7 @@ __global__ __launch_bounds__(256) void k_sample_short(SampleArgs g) {
         if (k == pick) {
             own = part[k];
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = w[k][e];
+            for (int e = 0; e < N; ++e) v[e] = q.w[k][e];
         }
     const double upto = before + group_scan<G>(own);
     const uint64_t over = __ballot(own > 0.0 && upto > aim) & group, some = __ballot(own > 0.0) & group;
@@ -419,13 +565,13 @@ __global__ __launch_bounds__(256) void k_sample_short(SampleArgs g) {
     for (int e = 0; e < N; ++e) {
         sum += v[e];
         if (open && v[e] > 0.0) {
-            found = (pick * G + lane) * N - r.shift + e;
+            found = q.place(pick, e);
             found_w = v[e];
             open = !(sum > aim);
         }
     }
-    g.actions[mine] = good ? found : -1;
-    g.log_prob[mine] = good ? (float)log(found_w / mass) : broken ? __builtin_nanf("") : 0.0f;
+    g.actions[mine] = q.good ? found : -1;
+    g.log_prob[mine] = q.good ? (float)log(found_w / mass) : broken ? __builtin_nanf("") : 0.0f;
 }
 
 // Longer rows: a block a row.  Each wave owns a contiguous piece of the row, so that running sums follow the index; of it every
@@ -438,34 +584,39 @@ __global__ __launch_bounds__(256) void k_sample_short(SampleArgs g) {
 // it (flat rows), the border is searched over the whole row.
 template <typename T, bool MASK, int THREADS, int H>
 struct LongRow {
-    static constexpr int N = Chunk<T>::N, W = THREADS / 64;
+    static constexpr int N = Chunk<T>::N, W = THREADS / 64, size = THREADS, buckets = 4 * THREADS, capacity = THREADS;
     struct Shared {
         double d[W + 1];
         int n[W + 1];
         float f[W];
         union {
             struct { float top[THREADS]; } maxima;
-            struct { uint64_t key[THREADS]; float x[THREADS]; } list;
+            struct { uint64_t key[THREADS]; } list;
         };
+        uint32_t hist[4 * THREADS];
+        Border border;
         float bound;
         int found, last;
     };
     const Row<T> r;
     Shared& sh;
-    const int tid, lane, wave, steps, first, end;      // chunks of this wave: first + 64 step + lane < end
+    const Settings& s;
+    const int tid, lane, wave, steps;                  // chunks of a wave: (wave steps + step) 64 + lane
+    const int rank;
+    uint32_t* const hist;
     Chunk<T> held[H];
     float m;
 
-    MDP_DEV LongRow(const SampleArgs& g, int64_t row, Shared& shared)
-        : r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row), sh(shared), tid(threadIdx.x), lane(threadIdx.x & 63),
-          wave(threadIdx.x >> 6), steps((r.chunks() + THREADS - 1) / THREADS), first(wave * steps * 64),
-          end(min(first + steps * 64, r.chunks())) {
+    MDP_DEV LongRow(const SampleArgs& g, int64_t row, const Settings& settings, Shared& shared)
+        : r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row), sh(shared), s(settings), tid(threadIdx.x), lane(threadIdx.x & 63),
+          wave(threadIdx.x >> 6), steps((r.chunks() + THREADS - 1) / THREADS), rank(threadIdx.x), hist(shared.hist) {
 #pragma unroll
-        for (int h = 0; h < H; ++h) held[h] = chunk(h);
+        for (int h = 0; h < H; ++h) held[h] = chunk(wave, h);
     }
-    MDP_DEV Chunk<T> chunk(int step) const {
-        const int j = first + 64 * step + lane;
-        if (step >= steps || j >= end) return Chunk<T>::lowest();
+    MDP_DEV int place(int of, int step) const { return ((of * steps + step) * 64 + lane) * N - r.shift; }
+    MDP_DEV Chunk<T> chunk(int of, int step) const {   // of wave `of`'s piece
+        const int j = (of * steps + step) * 64 + lane;
+        if (step >= steps || j >= r.chunks()) return Chunk<T>::lowest();
         if (!MASK && r.full(j)) return r.chunk(j);
         float v[N];
         r.template load<MASK>(j, v);
@@ -473,7 +624,7 @@ struct LongRow {
     }
     // f(step, entries) for each of this thread's chunks
     template <class F>
-    MDP_DEV void each(F&& f) const {
+    MDP_DEV void each_chunk(F&& f) const {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             if (h < steps) {
@@ -484,27 +635,38 @@ struct LongRow {
             }
             __builtin_amdgcn_sched_barrier(0);         // one chunk's arithmetic at a time: all of them at once would not fit the registers
         }
-        for (int h = H; h < steps; ++h) {
-            const Chunk<T> q = chunk(h);
-            float v[N];
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = q.at(e);
-            f(h, v);
-        }
+        each_chunk_again(f, H);
     }
-    // the same with every chunk read again: for what is asked of a whole row only where the candidates do not decide.  A loop, where
-    // the registers would need the code once for each chunk that they hold.
+    // the same with every chunk read again: a loop, where the registers would need the code once for each chunk that they hold
     template <class F>
-    MDP_DEV void each_again(F&& f) const {
-        for (int h = 0; h < steps; ++h) {
-            const Chunk<T> q = chunk(h);
+    MDP_DEV void each_chunk_again(F&& f, int from = 0) const {
+        for (int h = from; h < steps; ++h) {
+            const Chunk<T> q = chunk(wave, h);
             float v[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) v[e] = q.at(e);
             f(h, v);
         }
     }
-    MDP_DEV double block_sum(double v) {
+    // what find_border asks for
+    template <class F>
+    MDP_DEV void each(F&& f) const {
+        each_chunk_again([&](int step, const float (&v)[N]) {
+            const int i0 = place(wave, step);
+#pragma unroll
+            for (int e = 0; e < N; ++e) f(v[e], i0 + e, [&] { return s.weight(v[e], m); });
+        });
+    }
+    MDP_DEV double weight(float x) const { return s.weight(x, m); }
+    MDP_DEV void sync() const { __syncthreads(); }
+    MDP_DEV bool any(bool v) const { return v; }       // the same for the whole block
+    MDP_DEV double sum(double v) const { return block_sum(v); }
+    MDP_DEV int sum(int v) const { return block_sum(v); }
+    MDP_DEV float highest(float v) const { return block_max(v); }
+    MDP_DEV float lowest(float v) const { return -block_max(-v); }
+    MDP_DEV double scan(double v) const { double all; return block_scan(v, all); }
+
+    MDP_DEV double block_sum(double v) const {
         v = group_sum<64>(v);
         __syncthreads();
         if (lane == 0) sh.d[wave] = v;
@@ -513,7 +675,7 @@ struct LongRow {
         for (int w = 0; w < W; ++w) t += sh.d[w];
         return t;
     }
-    MDP_DEV int block_sum(int v) {
+    MDP_DEV int block_sum(int v) const {
         v = group_sum<64>(v);
         __syncthreads();
         if (lane == 0) sh.n[wave] = v;
@@ -522,7 +684,7 @@ struct LongRow {
         for (int w = 0; w < W; ++w) t += sh.n[w];
         return t;
     }
-    MDP_DEV float block_max(float v) {
+    MDP_DEV float block_max(float v) const {
         v = group_max<64>(v);
         __syncthreads();
         if (lane == 0) sh.f[wave] = v;
@@ -532,7 +694,7 @@ struct LongRow {
         return t;
     }
     // sum over the threads up to and with this one; `all` over every thread
-    MDP_DEV double block_scan(double v, double& all) {
+    MDP_DEV double block_scan(double v, double& all) const {
         v = group_scan<64>(v);
         __syncthreads();
         if (lane == 63) sh.d[wave] = v;
@@ -545,17 +707,14 @@ struct LongRow {
         }
         return before + v;
     }
-    MDP_DEV double exact_mass(const Settings& s) {
+    MDP_DEV double exact_mass() const {
         double t = 0.0;
-        each_again([&](int, const float (&v)[N]) {
-#pragma unroll
-            for (int e = 0; e < N; ++e) t += s.weight(v[e], m);
-        });
+        each([&](float, int, auto&& w) { t += w(); });
         return block_sum(t);
     }
 
     // A value not above the border, from the threads' largest entries, or -inf.  `mass`: the row's, in 32 bits.
-    MDP_DEV float bound_of(const Settings& s, float top, float mass) {
+    MDP_DEV float bound_of(float top, float mass) const {
         __syncthreads();
         sh.maxima.top[tid] = top;
         __syncthreads();
@@ -598,13 +757,15 @@ struct LongRow {
         return sh.bound;
     }
 
-    // Gathers the entries >= bound in index order (position in the row beside each); their number, or -1 if there are too many.
-    MDP_DEV int gather(float bound) {
+    // Gathers the entries that p names as words that sort by (value falling, place rising); their number, or -1 if there are too many.
+    template <bool AGAIN, class P>
+    MDP_DEV int gather_words(P&& p) const {
         int mine = 0;
-        each([&](int, const float (&v)[N]) {
+        const auto count = [&](int, const float (&v)[N]) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) mine += v[e] >= bound;
-        });
+            for (int e = 0; e < N; ++e) mine += p(v[e]);
+        };
+        if constexpr (AGAIN) each_chunk_again(count); else each_chunk(count);
         mine = group_sum<64>(mine);
         __syncthreads();
         if (lane == 0) sh.n[wave] = mine;
@@ -615,30 +776,73 @@ struct LongRow {
             total += sh.n[w];
         }
         if (total > THREADS) return -1;
-        each([&](int step, const float (&v)[N]) {
+        const auto put = [&](int step, const float (&v)[N]) {
             int n = 0;
 #pragma unroll
-            for (int e = 0; e < N; ++e) n += v[e] >= bound;
+            for (int e = 0; e < N; ++e) n += p(v[e]);
             if (__any(n)) {
                 const int upto = group_scan<64>(n);
                 int to = base + upto - n;
-                const int i0 = (first + 64 * step + lane) * N - r.shift;
+                const int i0 = place(wave, step);
 #pragma unroll
                 for (int e = 0; e < N; ++e)
-                    if (v[e] >= bound) {
-                        sh.list.x[to] = v[e] + 0.0f;
-                        sh.list.key[to] = (uint64_t)(~key_of(v[e])) << 32 | (uint32_t)(i0 + e);
-                        ++to;
-                    }
-                base += __shfl(upto, 63);
+                    if (p(v[e])) sh.list.key[to++] = (uint64_t)(~key_of(v[e])) << 32 | (uint32_t)(i0 + e);
+                base += of_lane(upto, 63);
             }
-        });
+        };
+        if constexpr (AGAIN) each_chunk_again(put); else each_chunk(put);
         __syncthreads();
         return total;
     }
+    MDP_DEV static float value_of(uint64_t word) { return of_key(~(uint32_t)(word >> 32)); }
+    template <bool COUNT, class P>
+    MDP_DEV void gather(P&& p) const { gather_words<true>(p); }
+    template <bool COUNT>
+    MDP_DEV Border last_kept(int n, double above, double aim) const {
+        const uint64_t word = tid < n ? sh.list.key[tid] : ~0ull;
+        __syncthreads();
+        const uint64_t sorted = sort(word, n);
+        const double v = tid < n ? (COUNT ? 1.0 : s.weight(value_of(sorted), m)) : 0.0;
+        double all;
+        const double before = above + (block_scan(v, all) - v);
+        const int kept = max(1, block_sum((int)(tid < n && before < aim)));
+        if (tid == kept - 1) sh.border = Border{value_of(sorted), (int)(uint32_t)sorted};
+        __syncthreads();
+        return sh.border;
+    }
+    MDP_DEV int nth_equal(float x, int r) const {
+        int mine = 0;
+        each([&](float v, int, auto&&) { mine += v == x; });
+        mine = group_sum<64>(mine);
+        __syncthreads();
+        if (lane == 0) sh.n[wave] = mine;
+        __syncthreads();
+        int seen = 0;
+        for (int w = 0; w < wave; ++w) seen += sh.n[w];
+        if (seen < r && seen + mine >= r)
+            each_chunk_again([&](int step, const float (&v)[N]) {
+                int equal = 0;
+#pragma unroll
+                for (int e = 0; e < N; ++e) equal += v[e] == x;
+                const int upto = group_scan<64>(equal);
+                int rank_of = seen + upto - equal;
+                seen += of_lane(upto, 63);
+                const int i0 = place(wave, step);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    rank_of += v[e] == x;
+                    if (v[e] == x && rank_of == r) sh.found = i0 + e;
+                }
+            });
+        __syncthreads();
+        return sh.found;
+    }
 
     // sorts the threads' words, rising with the thread
-    MDP_DEV uint64_t sort(uint64_t v, int n) {
+    MDP_DEV uint64_t sort(uint64_t v, int n) const {
+        int padded = 64;
+        while (padded < n) padded <<= 1;
+        n = padded;
         for (int size = 2; size < 2 * n; size <<= 1)
             for (int stride = size >> 1; stride; stride >>= 1) {
                 uint64_t o;
@@ -655,25 +859,18 @@ struct LongRow {
         return v;
     }
 
-    MDP_DEV void answer(const SampleArgs& g, int64_t row, int i, double w, double mass) {
+    MDP_DEV void answer(const SampleArgs& g, int64_t row, int i, double w, double mass) const {
         g.actions[row] = i;
         g.log_prob[row] = (float)log(w / mass);
     }
 
     // the draw among n gathered candidates, among which is everything that k, p and min_p keep
-    MDP_DEV void draw_from_list(const SampleArgs& g, int64_t row, const Settings& s, int n, double mass32) {
-        const bool in = tid < n;
-        const float x = in ? sh.list.x[tid] : 0.0f;
-        const uint64_t word = in ? sh.list.key[tid] : ~0ull;
-        const double w = in ? s.weight(x, m) : 0.0;
-        int padded = 64;
-        while (padded < n) padded <<= 1;
+    MDP_DEV void draw_from_list(const SampleArgs& g, int64_t row, int n, double mass32) const {
+        const uint64_t word = tid < n ? sh.list.key[tid] : ~0ull;
+        const double w = tid < n ? s.weight(value_of(word), m) : 0.0;
         __syncthreads();
-        // sorted by (value falling, place rising): the low half of the word is the place in the row; the thread's place in the
-        // list is found again through it below
-        const uint64_t sorted = sort(word, padded);
-        const bool in_s = tid < n;
-        const double ws = in_s ? s.weight(of_key(~(uint32_t)(sorted >> 32)), m) : 0.0;
+        const uint64_t sorted = sort(word, n);
+        const double ws = tid < n ? s.weight(value_of(sorted), m) : 0.0;
         double all;
         const double upto = block_scan(ws, all), before = upto - ws;
         int kept = s.k > 0 ? min(s.k, n) : n;
@@ -686,20 +883,20 @@ struct LongRow {
                 const int low = block_sum((int)(tid < kept && before < s.p * held * (1.0 - 7.7e-6)));
                 const int high = block_sum((int)(tid < kept && before < s.p * held * (1.0 + 7.7e-6)));
                 if (low != high) {
-                    held = exact_mass(s);
+                    held = exact_mass();
                     short_of = block_sum((int)(tid < kept && before < s.p * held));
                 }
             }
             kept = min(kept, short_of);
         }
-        kept = min(kept, block_sum((int)(in_s && ws >= s.mp)));
+        kept = min(kept, block_sum((int)(tid < n && ws >= s.mp)));
         kept = max(kept, 1);
-        // the lowest word that is not kept tells by itself which entries of the list are
+        // the word of the last one that is kept tells by itself which entries of the list are
         __syncthreads();
         if (tid == kept - 1) sh.list.key[0] = sorted;
         __syncthreads();
         const uint64_t border = sh.list.key[0];
-        const double kw = in && word <= border ? w : 0.0;
+        const double kw = tid < n && word <= border ? w : 0.0;
         double sum;
         const double line = block_scan(kw, sum);
         const double aim = s.u * sum;
@@ -714,83 +911,26 @@ struct LongRow {
         if (tid == who) answer(g, row, (int)(uint32_t)word, kw, sum);
     }
 
-    // the draw over the whole row
-    MDP_DEV void draw_from_row(const SampleArgs& g, int64_t row, const Settings& s) {
-        Border b{-__FLT_MAX__, 0x7fffffff, 0, 0.0, 0};
-        if (s.k > 0 || s.p < 1.0) {
-            const auto any = [](bool v) { return v; };
-            int allowed = 0;
-            each_again([&](int, const float (&v)[N]) {
+    MDP_DEV double kept_mass(const Border& b, int of, int step, double (&w)[N]) const {
+        const Chunk<T> q = chunk(of, step);
+        const int i0 = place(of, step);
+        double t = 0.0;
 #pragma unroll
-                for (int e = 0; e < N; ++e) allowed += v[e] > -kInf;
-            });
-            allowed = block_sum(allowed);
-            b = find_border(s, m, allowed, exact_mass(s),
-                [&](float from) {
-                    int n = 0;
-                    double q = 0.0;
-                    each_again([&](int, const float (&v)[N]) {
-#pragma unroll
-                        for (int e = 0; e < N; ++e) {
-                            const bool yes = v[e] >= from;
-                            n += yes;
-                            q += yes ? s.weight(v[e], m) : 0.0;
-                        }
-                    });
-                    const int count = block_sum(n);
-                    return Measure{count, block_sum(q)};
-                },
-                [&](float under) {
-                    float t = -kInf;
-                    each_again([&](int, const float (&v)[N]) {
-#pragma unroll
-                        for (int e = 0; e < N; ++e) t = v[e] < under ? larger(v[e], t) : t;
-                    });
-                    return block_max(t);
-                }, any);
+        for (int e = 0; e < N; ++e) {
+            w[e] = b.keeps(q.at(e), i0 + e) ? s.weight(q.at(e), m) : 0.0;
+            w[e] = w[e] >= s.mp ? w[e] : 0.0;
+            t += w[e];
         }
-        const bool ranked = b.room < b.level;
-        int rank0 = 0;
-        if (ranked) {
-            int equal = 0;
-            each_again([&](int, const float (&v)[N]) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) equal += v[e] == b.tau;
-            });
-            equal = group_sum<64>(equal);
-            __syncthreads();
-            if (lane == 0) sh.n[wave] = equal;
-            __syncthreads();
-            for (int w = 0; w < wave; ++w) rank0 += sh.n[w];
-        }
-        // f(step, kept weights) in index order; false ends it
-        const auto kept_weights = [&](int step, const float (&v)[N], int& rank, double (&w)[N]) {
-            int mine = 0;
-            if (ranked) {
-                int equal = 0;
-#pragma unroll
-                for (int e = 0; e < N; ++e) equal += v[e] == b.tau;
-                const int upto = group_scan<64>(equal);
-                mine = rank + upto - equal;
-                rank += __shfl(upto, 63);
-            }
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const bool equal = v[e] == b.tau;
-                const bool keep = v[e] > b.tau || (equal && (!ranked || mine < b.room));
-                mine += equal;
-                w[e] = keep ? s.weight(v[e], m) : 0.0;
-                w[e] = w[e] >= s.mp ? w[e] : 0.0;
-            }
-        };
+        return t;
+    }
+    // The draw over the whole row: the masses of the waves' pieces, then of the steps of the piece that holds the aim (a wave each),
+    // then the entries of that step.
+    MDP_DEV void draw_from_row(const SampleArgs& g, int64_t row, const Border& b) const {
         double mass = 0.0;
-        int rank = rank0;
-        each_again([&](int step, const float (&v)[N]) {
+        for (int h = 0; h < steps; ++h) {
             double w[N];
-            kept_weights(step, v, rank, w);
-#pragma unroll
-            for (int e = 0; e < N; ++e) mass += w[e];
-        });
+            mass += kept_mass(b, wave, h, w);
+        }
         mass = group_sum<64>(mass);
         __syncthreads();
         if (lane == 0) sh.d[wave] = mass;
@@ -798,45 +938,45 @@ struct LongRow {
         double total = 0.0, before = 0.0, run = 0.0;
         for (int w = 0; w < W; ++w) total += sh.d[w];
         const double aim = s.u * total;
-        int target = -1;
+        int target = 0;
         for (int w = 0; w < W; ++w) {
             if (sh.d[w] > 0.0 && run <= aim) { target = w; before = run; }
             run += sh.d[w];
         }
-        if (wave != target) return;
-        rank = rank0;
-        bool open = true;
-        int found = -1;
-        double found_w = 1.0;
-        each_again([&](int step, const float (&v)[N]) {
-            if (!open) return;                                         // uniform over the wave
-            double w[N], own = 0.0;
-            kept_weights(step, v, rank, w);
-#pragma unroll
-            for (int e = 0; e < N; ++e) own += w[e];
-            const double upto = before + group_scan<64>(own);
-            const uint64_t over = __ballot(own > 0.0 && upto > aim), some = __ballot(own > 0.0);
-            if (some) {                                                // see the short rows
-                const int winner = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
-                double sum = upto - own, my_w = 1.0;
-                int my = -1;
-                bool looking = true;
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    sum += w[e];
-                    if (looking && w[e] > 0.0) {
-                        my = (first + 64 * step + lane) * N - r.shift + e;
-                        my_w = w[e];
-                        looking = !(sum > aim);
-                    }
-                }
-                found = __shfl(my, winner);
-                found_w = __shfl(my_w, winner);
+        int at = 0;
+        run = before;
+        for (int h0 = 0; h0 < steps; h0 += W) {
+            double w[N];
+            const double part = group_sum<64>(kept_mass(b, target, h0 + wave, w));
+            __syncthreads();
+            if (lane == 0) sh.d[wave] = part;
+            __syncthreads();
+            for (int h = 0; h < W; ++h) {
+                if (sh.d[h] > 0.0 && run <= aim) { at = h0 + h; before = run; }
+                run += sh.d[h];
             }
-            open = over == 0ull;
-            before = __shfl(upto, 63);
-        });
-        if (lane == 0) answer(g, row, found, found_w, total);
+            if (run > aim) break;                      // uniform
+        }
+        if (wave) return;
+        double w[N];
+        const double own = kept_mass(b, target, at, w);
+        const double upto = before + group_scan<64>(own);
+        const uint64_t over = __ballot(own > 0.0 && upto > aim), some = __ballot(own > 0.0);
+        const int winner = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);   // see the short rows
+        if (lane != winner) return;
+        double sum = upto - own, found_w = 1.0;
+        int found = -1;
+        bool open = true;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            sum += w[e];
+            if (open && w[e] > 0.0) {
+                found = place(target, at) + e;
+                found_w = w[e];
+                open = !(sum > aim);
+            }
+        }
+        answer(g, row, found, found_w, total);
     }
 };
 
@@ -846,43 +986,53 @@ __global__ __launch_bounds__(THREADS) void k_sample_long(SampleArgs g) {
     constexpr int N = Chunk<T>::N;
     __shared__ typename L::Shared sh;
     const int64_t row = blockIdx.x;
-    L q(g, row, sh);
     const Settings s(g, row);
+    L q(g, row, s, sh);
     float top = -kInf;
-    q.each([&](int, const float (&v)[N]) {
+    int odd = 0;                                       // no distribution: a NaN or +inf
+    q.each_chunk([&](int, const float (&v)[N]) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) top = larger(v[e], top);
+        for (int e = 0; e < N; ++e) {
+            odd |= !(v[e] < kInf);
+            top = larger(v[e], top);
+        }
     });
     q.m = q.block_max(top);
-    const bool empty = q.m == -kInf;
-    // the row's mass in 32 bits, and whether it has a distribution at all
-    float mass = 0.0f;
-    const float c = s.c32();
-    q.each([&](int, const float (&v)[N]) {
-        float part = 0.0f;
-#pragma unroll
-        for (int e = 0; e < N; ++e) part += __builtin_amdgcn_exp2f((v[e] - q.m) * c);
-        mass += part;
-    });
-    const double total = q.block_sum((double)mass);
-    if (empty || !(total > 0.0) || s.c != s.c) {
+    const bool broken = __syncthreads_or(odd) != 0 || s.c != s.c;
+    if (broken || q.m == -kInf) {
         if (threadIdx.x == 0) {
             g.actions[row] = -1;
-            g.log_prob[row] = empty && s.c == s.c ? 0.0f : __builtin_nanf("");
+            g.log_prob[row] = broken ? __builtin_nanf("") : 0.0f;
         }
         return;
     }
+    Border b = everything();
     if (!s.all()) {
-        const float bound = q.bound_of(s, top, (float)total);
+        // the row's mass in 32 bits
+        float mass = 0.0f;
+        int allowed = 0;
+        const float c = s.c32();
+        q.each_chunk([&](int, const float (&v)[N]) {
+            float part = 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                part += __builtin_amdgcn_exp2f((v[e] - q.m) * c);
+                allowed += v[e] > -kInf;
+            }
+            mass += part;
+        });
+        const double total = q.block_sum((double)mass);
+        const float bound = q.bound_of(top, (float)total);
         if (bound > -kInf) {
-            const int n = q.gather(bound);
+            const int n = q.template gather_words<false>([&](float v) { return v >= bound; });
             if (n > 0) {
-                q.draw_from_list(g, row, s, n, total);
+                q.draw_from_list(g, row, n, total);
                 return;
             }
         }
+        if (s.k > 0 || s.p < 1.0) b = border_of(q, s, q.m, s.p < 1.0 ? q.exact_mass() : total, q.block_sum(allowed));
     }
-    q.draw_from_row(g, row, s);
+    q.draw_from_row(g, row, b);
 }
 
 __global__ void k_state_advance(unsigned long long* state) { state[1] += 1ull; }

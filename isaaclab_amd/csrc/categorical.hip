@@ -240,96 +240,99 @@ MDP_DEV void anew(V& x) { asm volatile("" : "+v"(x)); }
 
 // Finds the last entry of the shortest prefix that holds `aim`, counting entries (COUNT) or their weights.  C is what searches a row
 // together -- a group of lanes or a block -- and gives
-//   each(f): f(x, place, w) for each of this lane's entries, w() its weight; weight(x); sum, highest, lowest over all; scan: the sum
-//   over the lanes up to and with this one; sync; any: over the lanes that run this loop in step; size, rank: lanes and this lane's
-//   number; hist[buckets] in shared memory, and there a list of up to `capacity` entries: gather<COUNT>(p) fills it with those that p
-//   names, last_kept<COUNT>(n, above, aim) finds the border among its n, with `above` before them; nth_equal(x, r): the place of the
-//   r-th entry equal to x (r from 1).
-// Entries are counted into buckets that fall with the value: about the maximum first, a bucket a small part of a binary order of
+//   each(f): f(x, place, w) for each of this lane's entries, w() its weight; sort_in(bucket, f): f(bucket of x, w) for each, and
+//   each_sorted(bucket, f): f(x, place, w, bucket of x) after it; weight(x); sum, highest, lowest over all; scan: the sum over the
+//   lanes up to and with this one; sync; any: over the lanes that run this loop in step; size, rank: lanes and this lane's number;
+//   hist[4 size] in shared memory, and there a list of up to `capacity` entries: put<COUNT>(x, place, w) adds one, listed() tells how
+//   many were put, last_kept<COUNT>(n, above, aim) finds the border among the n listed, with `above` before them; nth_equal(x, r):
+//   the place of the r-th entry equal to x (r from 1).
+// Entries are sorted into buckets that fall with the value: about the maximum first, a bucket a small part of a binary order of
 // magnitude (entries below 24 of them share the last).  The bucket in which the aim is reached, by 32-bit fixed point, is confirmed
-// in 64 bits; its few entries are then looked at one by one.  If they are too many, the bucket is cut again, by keys, which ends
-// with one value.
+// in 64 bits while its few entries are listed, and these are looked at one by one.  If they are too many, the bucket is cut again,
+// by keys, which ends with one value.
 template <bool COUNT, class C>
 MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double total, bool active) {
+    constexpr int LAST = 4 * C::size - 2, NONE = 4 * C::size - 1;       // the last bucket; an entry that is in none
     Border border = everything();
-    float per = (float)C::buckets / 24.0f * s.c32();              // buckets for a difference of 1
-    double scale = COUNT ? 1.0 : 2147483648.0 / total;                 // all weights together: half of what 32 bits hold
+    float per = (float)LAST / 24.0f * s.c32();                          // buckets for a difference of 1
+    double scale = COUNT ? 1.0 : 2147483648.0 / total;                  // all weights together: half of what 32 bits hold
     float top = m, bottom = -__FLT_MAX__;
     double above = 0.0;
     int shift = -1;                                    // by value; later by key >> shift
-    const auto bucket = [&](float x) {
-        if (c.any(shift >= 0)) {
-            float again = x;
-            anew(again);
-            if (shift >= 0) return (int)((key_of(top) - key_of(again)) >> shift);
-        }
-        return (int)(uint32_t)fminf((top - x) * per, (float)(C::buckets - 1));
-    };
+    const auto by_value = [&](float x) { return x <= top && x >= bottom ? (int)fminf((top - x) * per, (float)LAST) : NONE; };
+    const auto by_key = [&](float x) { return x <= top && x >= bottom ? (int)((key_of(top) - key_of(x)) >> shift) : NONE; };
+    const auto bucket = [&](float x) { return shift < 0 ? by_value(x) : by_key(x); };
     while (c.any(active)) {
         c.sync();
-        for (int i = c.rank; i < C::buckets; i += C::size) c.hist[i] = 0u;
+        for (int i = 0; i < 4; ++i) c.hist[c.rank * 4 + i] = 0u;
         c.sync();
         anew(per);
         anew(scale);
-        c.each([&](float x, int, auto&& w) {
-            if (active && x <= top && x >= bottom) atomicAdd(&c.hist[bucket(x)], COUNT ? 1u : (uint32_t)fma(w(), scale, 0.5));
-        });
+        const auto count_in = [&](int b, auto&& w) {
+            if (active && b != NONE) atomicAdd(&c.hist[b], COUNT ? 1u : (uint32_t)fma(w(), scale, 0.5));
+        };
+        if (c.any(active && shift >= 0)) c.sort_in(bucket, count_in);
+        else c.sort_in(by_value, count_in);
         c.sync();
-        constexpr int PER = C::buckets / C::size;
-        const double need = (aim - above) * scale;
-        double mine = 0.0;
-        uint32_t q[PER];
+        const double need_d = fmin(fmax((aim - above) * scale, 1.0), 4294967295.0);
+        const uint32_t need = (uint32_t)__builtin_ceil(need_d);
+        uint32_t q[4], mine = 0u;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            q[i] = c.hist[c.rank * PER + i];
-            mine += (double)q[i];
+        for (int i = 0; i < 4; ++i) {
+            q[i] = c.hist[c.rank * 4 + i];
+            mine += q[i];
         }
-        double run = c.scan(mine) - mine;
-        int b = C::buckets;
+        uint32_t run = c.scan(mine) - mine;
+        int b = NONE, full = -1;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            run += (double)q[i];
-            if (b == C::buckets && run >= need && q[i]) b = c.rank * PER + i;
+        for (int i = 0; i < 4; ++i) {
+            run += q[i];
+            if (b == NONE && run >= need) b = c.rank * 4 + i;
+            if (q[i]) full = c.rank * 4 + i;
         }
         b = (int)c.lowest((float)b);
-        if (b == C::buckets) b = C::buckets - 1;
-        // confirm
+        if (c.any(active && b == NONE)) {              // the aim in the rounding of the last ones: the last that holds anything
+            full = (int)c.highest((float)full);
+            if (b == NONE) b = full < 0 ? LAST : full;
+        }
+        // confirm: the bucket is not the one while the entries above it reach the aim by themselves, or fall short of it with its own
         int count;
         double more;
-        bool sure = false;
-        do {
-            count = 0;
+        bool sure = !active, few = false;
+        for (;;) {
             more = 0.0;
             double in = 0.0;
-            anew(per);
-            c.each([&](float x, int, auto&& w) {
-                const int at = x <= top && x >= bottom ? bucket(x) : C::buckets;
+            c.sync();
+            c.clear_list();
+            c.sync();
+            c.each_sorted(bucket, [&](float x, int i, auto&& w, int at) {
                 const double v = COUNT ? 1.0 : w();
                 more += at < b ? v : 0.0;
-                in += at == b ? v : 0.0;
-                count += at == b;
+                if (at == b) {
+                    in += v;
+                    if (active) c.template put<COUNT>(x, i, v);
+                }
             });
-            count = c.sum(count);
+            c.sync();
             more = c.sum(more);
             in = c.sum(in);
+            count = c.listed();
             int to = b;
             if (above + more >= aim && b > 0) to = b - 1;
-            else if (above + more + in < aim && b < C::buckets - 1) to = b + 1;
+            else if (above + more + in < aim && b < LAST) to = b + 1;
             else sure = true;
-            b = to;
-        } while (c.any(active && !sure));
-        const bool few = count <= C::capacity;
-        anew(per);
+            if (!c.any(active && !sure)) break;
+            b = sure ? b : to;
+        }
+        few = count <= C::capacity;
         if (c.any(active && few)) {
-            c.template gather<COUNT>([&](float x) { return active && few && x <= top && x >= bottom && bucket(x) == b; });
             const Border found = c.template last_kept<COUNT>(active && few ? count : 0, above + more, aim);
             if (active && few) border = found;
         }
         if (c.any(active && !few)) {
             float hi = -kInf, lo = kInf;
-            anew(per);
-            c.each([&](float x, int, auto&&) {
-                if (x <= top && x >= bottom && bucket(x) == b) { hi = fmaxf(hi, x); lo = fminf(lo, x); }
+            c.each_sorted(bucket, [&](float x, int, auto&&, int at) {
+                if (at == b) { hi = fmaxf(hi, x); lo = fminf(lo, x); }
             });
             hi = c.highest(hi);
             lo = c.lowest(lo);
@@ -346,7 +349,7 @@ MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double 
                 above += more;
                 const uint32_t range = key_of(hi) - key_of(lo);
                 shift = 0;
-                while (range >> shift >= (uint32_t)C::buckets) ++shift;
+                while (range >> shift > (uint32_t)LAST) ++shift;
             }
             active = active && !few && !one;
         } else active = false;
@@ -387,8 +390,8 @@ MDP_DEV void wave_sync() {
 // through their loops together until the last is done.
 template <typename T, int G, int K>
 struct ShortRow {
-    static constexpr int N = Chunk<T>::N, size = G, buckets = 4 * G, capacity = G;
-    struct Shared { uint32_t hist[buckets]; float x[G]; int place[G]; double value[G]; };
+    static constexpr int N = Chunk<T>::N, size = G, capacity = G;
+    struct Shared { uint32_t hist[4 * G]; double value[G]; float x[G]; int place[G]; int n; };
     float x[K][N];
     double w[K][N];
     int rank, shift;                                   // this lane's number; the row's shift
@@ -415,21 +418,43 @@ struct ShortRow {
     template <typename V> MDP_DEV V scan(V v) const { return group_scan<G>(v); }
     MDP_DEV void sync() const { wave_sync(); }
     MDP_DEV bool any(bool v) const { return __any(v && good) != 0; }
-    template <bool COUNT, class P>
-    MDP_DEV void gather(P&& p) const {
-        int n = 0;
-        each([&](float v, int, auto&&) { n += p(v); });
-        int to = scan(n) - n;
-        if (n)
-            each([&](float v, int i, auto&& w) {
-                if (p(v)) {
-                    sh->x[to] = v;
-                    sh->place[to] = i;
-                    sh->value[to] = COUNT ? 1.0 : w();
-                    ++to;
-                }
-            });
-        sync();
+    // the buckets of the entries, a byte each
+    uint32_t ids[4];
+    template <class B, class F>
+    MDP_DEV void sort_in(B&& bucket, F&& f) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            uint32_t four = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = (4 * q + e) / N, l = (4 * q + e) % N;
+                const int b = bucket(x[k][l]);
+                four |= (uint32_t)b << 8 * e;
+                f(b, [&] { return w[k][l]; });
+            }
+            ids[q] = four;
+        }
+    }
+    template <class B, class F>
+    MDP_DEV void each_sorted(B&&, F&& f) const {
+        int base = rank * N - shift;
+        anew(base);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int k = i / N, l = i % N;
+            f(x[k][l], base + k * G * N + l, [&] { return w[k][l]; }, (int)(ids[i / 4] >> 8 * (i % 4) & 0xffu));
+        }
+    }
+    MDP_DEV void clear_list() const { if (rank == 0) sh->n = 0; }
+    MDP_DEV int listed() const { return sh->n; }
+    template <bool COUNT>
+    MDP_DEV void put(float v, int i, double value) const {
+        const int to = atomicAdd(&sh->n, 1);           // in any order: what is asked of the list goes by value and place
+        if (to < capacity) {
+            sh->x[to] = v;
+            sh->place[to] = i;
+            sh->value[to] = value;
+        }
     }
     template <bool COUNT>
     MDP_DEV Border last_kept(int n, double above, double aim) const {
@@ -584,7 +609,7 @@ __global__ __launch_bounds__(256, 4) void k_sample_short(SampleArgs g) {
 // it (flat rows), the border is searched over the whole row.
 template <typename T, bool MASK, int THREADS, int H>
 struct LongRow {
-    static constexpr int N = Chunk<T>::N, W = THREADS / 64, size = THREADS, buckets = 4 * THREADS, capacity = THREADS;
+    static constexpr int N = Chunk<T>::N, W = THREADS / 64, size = THREADS, capacity = THREADS;
     struct Shared {
         double d[W + 1];
         int n[W + 1];
@@ -596,7 +621,7 @@ struct LongRow {
         uint32_t hist[4 * THREADS];
         Border border;
         float bound;
-        int found, last;
+        int found, last, listed;
     };
     const Row<T> r;
     Shared& sh;
@@ -664,7 +689,14 @@ struct LongRow {
     MDP_DEV int sum(int v) const { return block_sum(v); }
     MDP_DEV float highest(float v) const { return block_max(v); }
     MDP_DEV float lowest(float v) const { return -block_max(-v); }
-    MDP_DEV double scan(double v) const { double all; return block_scan(v, all); }
+    MDP_DEV uint32_t scan(uint32_t v) const {
+        v = group_scan<64>(v);
+        __syncthreads();
+        if (lane == 63) sh.n[wave] = (int)v;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) v += (uint32_t)sh.n[w];
+        return v;
+    }
 
     MDP_DEV double block_sum(double v) const {
         v = group_sum<64>(v);
@@ -758,14 +790,13 @@ struct LongRow {
     }
 
     // Gathers the entries that p names as words that sort by (value falling, place rising); their number, or -1 if there are too many.
-    template <bool AGAIN, class P>
+    template <class P>
     MDP_DEV int gather_words(P&& p) const {
         int mine = 0;
-        const auto count = [&](int, const float (&v)[N]) {
+        each_chunk([&](int, const float (&v)[N]) {
 #pragma unroll
             for (int e = 0; e < N; ++e) mine += p(v[e]);
-        };
-        if constexpr (AGAIN) each_chunk_again(count); else each_chunk(count);
+        });
         mine = group_sum<64>(mine);
         __syncthreads();
         if (lane == 0) sh.n[wave] = mine;
@@ -776,7 +807,7 @@ struct LongRow {
             total += sh.n[w];
         }
         if (total > THREADS) return -1;
-        const auto put = [&](int step, const float (&v)[N]) {
+        each_chunk([&](int step, const float (&v)[N]) {
             int n = 0;
 #pragma unroll
             for (int e = 0; e < N; ++e) n += p(v[e]);
@@ -789,14 +820,26 @@ struct LongRow {
                     if (p(v[e])) sh.list.key[to++] = (uint64_t)(~key_of(v[e])) << 32 | (uint32_t)(i0 + e);
                 base += of_lane(upto, 63);
             }
-        };
-        if constexpr (AGAIN) each_chunk_again(put); else each_chunk(put);
+        });
         __syncthreads();
         return total;
     }
     MDP_DEV static float value_of(uint64_t word) { return of_key(~(uint32_t)(word >> 32)); }
-    template <bool COUNT, class P>
-    MDP_DEV void gather(P&& p) const { gather_words<true>(p); }
+    template <class B, class F>
+    MDP_DEV void sort_in(B&& bucket, F&& f) const {
+        each([&](float x, int, auto&& w) { f(bucket(x), w); });
+    }
+    template <class B, class F>
+    MDP_DEV void each_sorted(B&& bucket, F&& f) const {
+        each([&](float x, int i, auto&& w) { f(x, i, w, bucket(x)); });
+    }
+    MDP_DEV void clear_list() const { if (tid == 0) sh.listed = 0; }
+    MDP_DEV int listed() const { return sh.listed; }
+    template <bool COUNT>
+    MDP_DEV void put(float x, int i, double) const {
+        const int to = atomicAdd(&sh.listed, 1);       // in any order: it is sorted
+        if (to < capacity) sh.list.key[to] = (uint64_t)(~key_of(x)) << 32 | (uint32_t)i;
+    }
     template <bool COUNT>
     MDP_DEV Border last_kept(int n, double above, double aim) const {
         const uint64_t word = tid < n ? sh.list.key[tid] : ~0ull;
@@ -1024,7 +1067,7 @@ __global__ __launch_bounds__(THREADS) void k_sample_long(SampleArgs g) {
         const double total = q.block_sum((double)mass);
         const float bound = q.bound_of(top, (float)total);
         if (bound > -kInf) {
-            const int n = q.template gather_words<false>([&](float v) { return v >= bound; });
+            const int n = q.gather_words([&](float v) { return v >= bound; });
             if (n > 0) {
                 q.draw_from_list(g, row, n, total);
                 return;

@@ -243,18 +243,19 @@ MDP_DEV void anew(V& x) { asm volatile("" : "+v"(x)); }
 //   each(f): f(x, place, w) for each of this lane's entries, w() its weight; sort_in(bucket, f): f(bucket of x, w) for each, and
 //   each_sorted(bucket, f): f(x, place, w, bucket of x) after it; weight(x); sum, highest, lowest over all; scan: the sum over the
 //   lanes up to and with this one; sync; any: over the lanes that run this loop in step; size, rank: lanes and this lane's number;
-//   hist[4 size] in shared memory, and there a list of up to `capacity` entries: put<COUNT>(x, place, w) adds one, listed() tells how
+//   hist[per_lane size] in shared memory, and there a list of up to `capacity` entries: put<COUNT>(x, place, w) adds one, listed() tells how
 //   many were put, last_kept<COUNT>(n, above, aim) finds the border among the n listed, with `above` before them; nth_equal(x, r):
 //   the place of the r-th entry equal to x (r from 1).
 // Entries are sorted into buckets that fall with the value: about the maximum first, a bucket a small part of a binary order of
-// magnitude (entries below 24 of them share the last).  The bucket in which the aim is reached, by 32-bit fixed point, is confirmed
+// magnitude or of what the row spans (entries more than `window` orders below share the last); bottom: the row's lowest entry.  The bucket in which the aim is reached, by 32-bit fixed point, is confirmed
 // in 64 bits while its few entries are listed, and these are looked at one by one.  If they are too many, the bucket is cut again,
 // by keys, which ends with one value.
 template <bool COUNT, class C>
 MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double total, bool active) {
-    constexpr int LAST = 4 * C::size - 2, NONE = 4 * C::size - 1;       // the last bucket; an entry that is in none
+    constexpr int PER = C::per_lane, LAST = PER * C::size - 2, NONE = PER * C::size - 1;   // the last bucket; an entry that is in none
     Border border = everything();
-    float per = (float)LAST / 24.0f * s.c32();                          // buckets for a difference of 1
+    aim = fmax(aim, 1e-300);                           // the first entry reaches a share of 0
+    float per = (float)LAST / fmaxf(fminf(C::window / s.c32(), m - c.bottom), 1e-30f);   // buckets for a difference of 1
     double scale = COUNT ? 1.0 : 2147483648.0 / total;                  // all weights together: half of what 32 bits hold
     float top = m, bottom = -__FLT_MAX__;
     double above = 0.0;
@@ -264,7 +265,7 @@ MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double 
     const auto bucket = [&](float x) { return shift < 0 ? by_value(x) : by_key(x); };
     while (c.any(active)) {
         c.sync();
-        for (int i = 0; i < 4; ++i) c.hist[c.rank * 4 + i] = 0u;
+        for (int i = 0; i < PER; ++i) c.hist[c.rank * PER + i] = 0u;
         c.sync();
         anew(per);
         anew(scale);
@@ -276,19 +277,19 @@ MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double 
         c.sync();
         const double need_d = fmin(fmax((aim - above) * scale, 1.0), 4294967295.0);
         const uint32_t need = (uint32_t)__builtin_ceil(need_d);
-        uint32_t q[4], mine = 0u;
+        uint32_t q[PER], mine = 0u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            q[i] = c.hist[c.rank * 4 + i];
+        for (int i = 0; i < PER; ++i) {
+            q[i] = c.hist[c.rank * PER + i];
             mine += q[i];
         }
         uint32_t run = c.scan(mine) - mine;
         int b = NONE, full = -1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < PER; ++i) {
             run += q[i];
-            if (b == NONE && run >= need) b = c.rank * 4 + i;
-            if (q[i]) full = c.rank * 4 + i;
+            if (b == NONE && run >= need) b = c.rank * PER + i;
+            if (q[i]) full = c.rank * PER + i;
         }
         b = (int)c.lowest((float)b);
         if (c.any(active && b == NONE)) {              // the aim in the rounding of the last ones: the last that holds anything
@@ -391,14 +392,16 @@ MDP_DEV void wave_sync() {
 template <typename T, int G, int K>
 struct ShortRow {
     static constexpr int N = Chunk<T>::N, size = G, capacity = G;
-    struct Shared { uint32_t hist[4 * G]; double value[G]; float x[G]; int place[G]; int n; };
+    static constexpr int per_lane = G < 8 ? 16 : G < 32 ? 8 : 4;
+    static constexpr float window = 14.0f;
+    struct Shared { uint32_t hist[per_lane * G]; double value[G]; float x[G]; int place[G]; int n; };
     float x[K][N];
     double w[K][N];
     int rank, shift;                                   // this lane's number; the row's shift
     uint32_t* hist;
     Shared* sh;
     bool good;
-    float m;
+    float m, bottom;
     const Settings* s;
 
     MDP_DEV int place(int k, int e) const { return (k * G + rank) * N - shift + e; }
@@ -534,15 +537,19 @@ __global__ __launch_bounds__(256, 4) void k_sample_short(SampleArgs g) {
     if (q.any(!s.all())) {
         double total = 0.0;
         int allowed = 0;
+        q.bottom = m;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 total += q.w[k][e];
-                allowed += q.x[k][e] > -kInf;
+                const bool is = q.x[k][e] > -kInf;
+                allowed += is;
+                q.bottom = is ? fminf(q.x[k][e], q.bottom) : q.bottom;
             }
         total = group_sum<G>(total);
         allowed = group_sum<G>(allowed);
+        q.bottom = q.lowest(q.bottom);
         const Border b = border_of(q, s, m, total, allowed);
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -610,6 +617,8 @@ __global__ __launch_bounds__(256, 4) void k_sample_short(SampleArgs g) {
 template <typename T, bool MASK, int THREADS, int H>
 struct LongRow {
     static constexpr int N = Chunk<T>::N, W = THREADS / 64, size = THREADS, capacity = THREADS;
+    static constexpr int per_lane = 4;
+    static constexpr float window = 24.0f;
     struct Shared {
         double d[W + 1];
         int n[W + 1];
@@ -618,7 +627,7 @@ struct LongRow {
             struct { float top[THREADS]; } maxima;
             struct { uint64_t key[THREADS]; } list;
         };
-        uint32_t hist[4 * THREADS];
+        uint32_t hist[per_lane * THREADS];
         Border border;
         float bound;
         int found, last, listed;
@@ -630,7 +639,7 @@ struct LongRow {
     const int rank;
     uint32_t* const hist;
     Chunk<T> held[H];
-    float m;
+    float m, bottom;
 
     MDP_DEV LongRow(const SampleArgs& g, int64_t row, const Settings& settings, Shared& shared)
         : r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row), sh(shared), s(settings), tid(threadIdx.x), lane(threadIdx.x & 63),
@@ -1055,6 +1064,7 @@ __global__ __launch_bounds__(THREADS) void k_sample_long(SampleArgs g) {
         float mass = 0.0f;
         int allowed = 0;
         const float c = s.c32();
+        q.bottom = -__FLT_MAX__;                       // not looked for: the window decides
         q.each_chunk([&](int, const float (&v)[N]) {
             float part = 0.0f;
 #pragma unroll

@@ -104,6 +104,7 @@ struct Row {
 
 // the larger of two numbers, b where a is a NaN (one instruction, without fmaxf's canonicalisation of its operands)
 MDP_DEV float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, kInf); }
+MDP_DEV float smaller(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, -kInf); }
 
 // lane i gets lane i ^ M's value (M < 4), for M = 4 and 8 that of the lane mirrored inside 8 or 16, for M = 16 and 32 that of a
 // lane in the other half of 32 or 64: what a reduction needs whose groups of M already agree
@@ -234,6 +235,10 @@ struct Border {
 };
 MDP_DEV Border everything() { return Border{-__FLT_MAX__, 0x7fffffff}; }
 
+// an entry as a word that rises in the order (value falling, place rising)
+MDP_DEV uint64_t word_of(float x, int place) { return (uint64_t)(~key_of(x)) << 32 | (uint32_t)place; }
+MDP_DEV float value_of(uint64_t word) { return of_key(~(uint32_t)(word >> 32)); }
+
 // Nothing that is computed from x before is kept for after this: sixteen entries' worth of it would not fit the registers
 template <typename V>
 MDP_DEV void anew(V& x) { asm volatile("" : "+v"(x)); }
@@ -260,9 +265,13 @@ MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double 
     float top = m, bottom = -__FLT_MAX__;
     double above = 0.0;
     int shift = -1;                                    // by value; later by key >> shift
-    const auto by_value = [&](float x) { return x <= top && x >= bottom ? (int)fminf((top - x) * per, (float)LAST) : NONE; };
-    const auto by_key = [&](float x) { return x <= top && x >= bottom ? (int)((key_of(top) - key_of(x)) >> shift) : NONE; };
-    const auto bucket = [&](float x) { return shift < 0 ? by_value(x) : by_key(x); };
+    const auto by_value = [&](float x) { return x > -kInf ? (int)fminf((top - x) * per, (float)LAST) : NONE; };
+    const auto bucket = [&](float x) {
+        if (shift < 0) return by_value(x);
+        float again = x;
+        anew(again);
+        return x <= top && x >= bottom ? (int)((key_of(top) - key_of(again)) >> shift) : NONE;
+    };
     while (c.any(active)) {
         c.sync();
         for (int i = 0; i < PER; ++i) c.hist[c.rank * PER + i] = 0u;
@@ -394,7 +403,8 @@ struct ShortRow {
     static constexpr int N = Chunk<T>::N, size = G, capacity = G;
     static constexpr int per_lane = G < 8 ? 16 : G < 32 ? 8 : 4;
     static constexpr float window = 14.0f;
-    struct Shared { uint32_t hist[per_lane * G]; double value[G]; float x[G]; int place[G]; int n; };
+    struct Listed { uint64_t word; double value; };      // the word rises in the order
+    struct Shared { Listed list[G]; uint32_t hist[per_lane * G]; int n; };
     float x[K][N];
     double w[K][N];
     int rank, shift;                                   // this lane's number; the row's shift
@@ -452,30 +462,26 @@ struct ShortRow {
     MDP_DEV int listed() const { return sh->n; }
     template <bool COUNT>
     MDP_DEV void put(float v, int i, double value) const {
+        anew(v);
         const int to = atomicAdd(&sh->n, 1);           // in any order: what is asked of the list goes by value and place
-        if (to < capacity) {
-            sh->x[to] = v;
-            sh->place[to] = i;
-            sh->value[to] = value;
-        }
+        if (to < capacity) sh->list[to] = Listed{word_of(v, i), value};
     }
     template <bool COUNT>
     MDP_DEV Border last_kept(int n, double above, double aim) const {
         const bool in = rank < n;
-        const float v = in ? sh->x[rank] : 0.0f;
-        const int i = in ? sh->place[rank] : 0;
+        const uint64_t mine = in ? sh->list[rank].word : ~0ull;
         double before = above;
         int order = 0;
         for (int j = 0; __any(j < n); ++j) {
-            const float o = sh->x[j];                  // beyond n: of no effect
-            const bool first = j < n && (o > v || (o == v && sh->place[j] < i));
-            before += first ? sh->value[j] : 0.0;
+            const Listed o = sh->list[j];              // beyond n: what was there before
+            const bool first = j < n && o.word < mine;
+            before += first ? o.value : 0.0;
             order += first;
         }
         int kept = sum((int)(in && before < aim));
         kept = kept ? kept : 1;
         const bool me = in && order == kept - 1;
-        return Border{highest(me ? v : -kInf), sum(me ? i : 0)};
+        return Border{highest(me ? value_of(mine) : -kInf), sum(me ? (int)(uint32_t)mine : 0)};
     }
     MDP_DEV int nth_equal(float v, int r) const {
         int seen = 0, at = 0;
@@ -545,17 +551,24 @@ __global__ __launch_bounds__(256, 4) void k_sample_short(SampleArgs g) {
                 total += q.w[k][e];
                 const bool is = q.x[k][e] > -kInf;
                 allowed += is;
-                q.bottom = is ? fminf(q.x[k][e], q.bottom) : q.bottom;
+                q.bottom = smaller(is ? q.x[k][e] : m, q.bottom);
             }
         total = group_sum<G>(total);
         allowed = group_sum<G>(allowed);
         q.bottom = q.lowest(q.bottom);
-        const Border b = border_of(q, s, m, total, allowed);
+        if (q.any(s.k > 0 || s.p < 1.0)) {
+            const Border b = border_of(q, s, m, total, allowed);
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+            for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                q.w[k][e] = b.keeps(q.x[k][e], q.place(k, e)) && q.w[k][e] >= s.mp ? q.w[k][e] : 0.0;
+                for (int e = 0; e < N; ++e) q.w[k][e] = b.keeps(q.x[k][e], q.place(k, e)) ? q.w[k][e] : 0.0;
+        }
+        if (q.any(s.mp > 0.0)) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < N; ++e) q.w[k][e] = q.w[k][e] >= s.mp ? q.w[k][e] : 0.0;
+        }
     }
     // masses by chunk index; the chunk row k that holds the aim, the lane in it, the entry in that
     double part[K], mass = 0.0, sums[K];
@@ -826,14 +839,13 @@ struct LongRow {
                 const int i0 = place(wave, step);
 #pragma unroll
                 for (int e = 0; e < N; ++e)
-                    if (p(v[e])) sh.list.key[to++] = (uint64_t)(~key_of(v[e])) << 32 | (uint32_t)(i0 + e);
+                    if (p(v[e])) sh.list.key[to++] = word_of(v[e], i0 + e);
                 base += of_lane(upto, 63);
             }
         });
         __syncthreads();
         return total;
     }
-    MDP_DEV static float value_of(uint64_t word) { return of_key(~(uint32_t)(word >> 32)); }
     template <class B, class F>
     MDP_DEV void sort_in(B&& bucket, F&& f) const {
         each([&](float x, int, auto&& w) { f(bucket(x), w); });
@@ -847,7 +859,7 @@ struct LongRow {
     template <bool COUNT>
     MDP_DEV void put(float x, int i, double) const {
         const int to = atomicAdd(&sh.listed, 1);       // in any order: it is sorted
-        if (to < capacity) sh.list.key[to] = (uint64_t)(~key_of(x)) << 32 | (uint32_t)i;
+        if (to < capacity) sh.list.key[to] = word_of(x, i);
     }
     template <bool COUNT>
     MDP_DEV Border last_kept(int n, double above, double aim) const {

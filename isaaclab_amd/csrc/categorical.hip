@@ -254,9 +254,10 @@ MDP_DEV void anew(V& x) { asm volatile("" : "+v"(x)); }
 // Entries are sorted into buckets that fall with the value: about the maximum first, a bucket a small part of a binary order of
 // magnitude or of what the row spans (entries more than `window` orders below share the last); bottom: the row's lowest entry.  The bucket in which the aim is reached, by 32-bit fixed point, is confirmed
 // in 64 bits while its few entries are listed, and these are looked at one by one.  If they are too many, the bucket is cut again,
-// by keys, which ends with one value.
+// by keys, which ends with one value.  Where `total`, the mass of the row, is known in 32 bits only (C::total_known false) and the aim
+// is a share of it (share_of_total), the first pass sums it up in 64.
 template <bool COUNT, class C>
-MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double total, bool active) {
+MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double total, bool share_of_total, bool active) {
     constexpr int PER = C::per_lane, LAST = PER * C::size - 2, NONE = PER * C::size - 1;   // the last bucket; an entry that is in none
     Border border = everything();
     aim = fmax(aim, 1e-300);                           // the first entry reaches a share of 0
@@ -278,12 +279,19 @@ MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double 
         c.sync();
         anew(per);
         anew(scale);
+        double weighed = 0.0;
         const auto count_in = [&](int b, auto&& w) {
-            if (active && b != NONE) atomicAdd(&c.hist[b], COUNT ? 1u : (uint32_t)fma(w(), scale, 0.5));
+            const double v = COUNT ? 1.0 : w();
+            if (!COUNT && !C::total_known) weighed += v;
+            if (active && b != NONE) atomicAdd(&c.hist[b], COUNT ? 1u : (uint32_t)fma(v, scale, 0.5));
         };
         if (c.any(active && shift >= 0)) c.sort_in(bucket, count_in);
         else c.sort_in(by_value, count_in);
         c.sync();
+        if (!COUNT && !C::total_known && share_of_total) {
+            aim = fmax(s.p * c.sum(weighed), 1e-300);
+            share_of_total = false;
+        }
         const double need_d = fmin(fmax((aim - above) * scale, 1.0), 4294967295.0);
         const uint32_t need = (uint32_t)__builtin_ceil(need_d);
         uint32_t q[PER], mine = 0u;
@@ -374,7 +382,7 @@ MDP_DEV Border border_of(C& c, const Settings& s, float m, double total, int all
     const bool by_k = s.k > 0 && s.k < allowed, by_p = s.p < 1.0;
     double held = total;
     if (c.any(by_k)) {
-        const Border f = find_border<true>(c, s, m, (double)s.k, 1.0, by_k);
+        const Border f = find_border<true>(c, s, m, (double)s.k, 1.0, false, by_k);
         if (by_k) b = f;
         if (c.any(by_k && by_p)) {
             double kept = 0.0;
@@ -383,7 +391,7 @@ MDP_DEV Border border_of(C& c, const Settings& s, float m, double total, int all
         }
     }
     if (c.any(by_p)) {
-        const Border f = find_border<false>(c, s, m, s.p * held, total, by_p);
+        const Border f = find_border<false>(c, s, m, s.p * held, total, !by_k, by_p);
         if (by_p && (f.tau > b.tau || (f.tau == b.tau && f.place < b.place))) b = f;
     }
     return b;
@@ -403,6 +411,7 @@ struct ShortRow {
     static constexpr int N = Chunk<T>::N, size = G, capacity = G;
     static constexpr int per_lane = G < 8 ? 16 : G < 32 ? 8 : 4;
     static constexpr float window = 14.0f;
+    static constexpr bool total_known = true;
     struct Listed { uint64_t word; double value; };      // the word rises in the order
     struct Shared { Listed list[G]; uint32_t hist[per_lane * G]; int n; };
     float x[K][N];
@@ -632,6 +641,7 @@ struct LongRow {
     static constexpr int N = Chunk<T>::N, W = THREADS / 64, size = THREADS, capacity = THREADS;
     static constexpr int per_lane = 4;
     static constexpr float window = 24.0f;
+    static constexpr bool total_known = false;
     struct Shared {
         double d[W + 1];
         int n[W + 1];
@@ -651,7 +661,7 @@ struct LongRow {
     const int tid, lane, wave, steps;                  // chunks of a wave: (wave steps + step) 64 + lane
     const int rank;
     uint32_t* const hist;
-    Chunk<T> held[H];
+    Chunk<T> held[H ? H : 1];
     float m, bottom;
 
     MDP_DEV LongRow(const SampleArgs& g, int64_t row, const Settings& settings, Shared& shared)
@@ -687,8 +697,10 @@ struct LongRow {
     // the same with every chunk read again: a loop, where the registers would need the code once for each chunk that they hold
     template <class F>
     MDP_DEV void each_chunk_again(F&& f, int from = 0) const {
+        Chunk<T> next = chunk(wave, from);
         for (int h = from; h < steps; ++h) {
-            const Chunk<T> q = chunk(wave, h);
+            const Chunk<T> q = next;
+            next = chunk(wave, h + 1);                 // on its way while this one is worked on
             float v[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) v[e] = q.at(e);
@@ -943,9 +955,9 @@ struct LongRow {
             if (s.k > 0) held = block_sum(tid == kept - 1 ? upto : 0.0);
             int short_of = block_sum((int)(tid < kept && before < s.p * held));
             if (s.k == 0) {
-                // the row's mass in 32 bits decides unless the border is within its error (2^-17) of the aim
-                const int low = block_sum((int)(tid < kept && before < s.p * held * (1.0 - 7.7e-6)));
-                const int high = block_sum((int)(tid < kept && before < s.p * held * (1.0 + 7.7e-6)));
+                // the row's mass in 32 bits decides unless the border is within its error (2^-16) of the aim
+                const int low = block_sum((int)(tid < kept && before < s.p * held * (1.0 - 1.53e-5)));
+                const int high = block_sum((int)(tid < kept && before < s.p * held * (1.0 + 1.53e-5)));
                 if (low != high) {
                     held = exact_mass();
                     short_of = block_sum((int)(tid < kept && before < s.p * held));
@@ -975,26 +987,38 @@ struct LongRow {
         if (tid == who) answer(g, row, (int)(uint32_t)word, kw, sum);
     }
 
-    MDP_DEV double kept_mass(const Border& b, int of, int step, double (&w)[N]) const {
-        const Chunk<T> q = chunk(of, step);
-        const int i0 = place(of, step);
+    MDP_DEV double kept_mass(const Border& b, const float (&v)[N], int i0, double (&w)[N]) const {
         double t = 0.0;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            w[e] = b.keeps(q.at(e), i0 + e) ? s.weight(q.at(e), m) : 0.0;
+            w[e] = b.keeps(v[e], i0 + e) ? s.weight(v[e], m) : 0.0;
             w[e] = w[e] >= s.mp ? w[e] : 0.0;
             t += w[e];
         }
         return t;
     }
+    MDP_DEV double kept_mass(const Border& b, int of, int step, double (&w)[N]) const {
+        const Chunk<T> q = chunk(of, step);
+        float v[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = q.at(e);
+        return kept_mass(b, v, place(of, step), w);
+    }
     // The draw over the whole row: the masses of the waves' pieces, then of the steps of the piece that holds the aim (a wave each),
     // then the entries of that step.
+    template <bool CUT>
     MDP_DEV void draw_from_row(const SampleArgs& g, int64_t row, const Border& b) const {
         double mass = 0.0;
-        for (int h = 0; h < steps; ++h) {
-            double w[N];
-            mass += kept_mass(b, wave, h, w);
-        }
+        if (!CUT)
+            each_chunk([&](int, const float (&v)[N]) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) mass += s.weight(v[e], m);
+            });
+        else
+            each_chunk_again([&](int h, const float (&v)[N]) {
+                double w[N];
+                mass += kept_mass(b, v, place(wave, h), w);
+            });
         mass = group_sum<64>(mass);
         __syncthreads();
         if (lane == 0) sh.d[wave] = mass;
@@ -1044,49 +1068,53 @@ struct LongRow {
     }
 };
 
+// While the row arrives: each thread's largest entry and its mass about that in 32 bits; then the row's.  False for a row without a
+// draw (answered here).  A NaN or +inf makes the mass a NaN.
+template <class L>
+MDP_DEV bool first_pass(L& q, const SampleArgs& g, int64_t row, float& top, double& total) {
+    constexpr int N = L::N;
+    const float c = q.s.c32();
+    top = -__FLT_MAX__;
+    float part = 0.0f;
+    q.each_chunk([&](int, const float (&v)[N]) {
+        float to = top;
+#pragma unroll
+        for (int e = 0; e < N; ++e) to = larger(v[e], to);
+        if (to > top) {
+            part *= __builtin_amdgcn_exp2f(larger((top - to) * c, -300.0f));
+            top = to;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum += __builtin_amdgcn_exp2f((v[e] - top) * c);
+        part += sum;
+    });
+    q.m = q.block_max(top);
+    total = q.block_sum((double)(part * __builtin_amdgcn_exp2f(larger((top - q.m) * c, -300.0f))));
+    const bool broken = total != total || q.s.c != q.s.c;
+    if (total > 0.0 && !broken) return true;
+    if (threadIdx.x == 0) {
+        g.actions[row] = -1;
+        g.log_prob[row] = broken ? __builtin_nanf("") : 0.0f;
+    }
+    return false;
+}
+
+constexpr int64_t kLeft = -2;                          // an action that is still to be drawn
+
+// Rows that k, p or min_p cut, by the list of candidates.  Rows that it does not decide are left to the kernel below: a kernel of its
+// own, so that what it needs does not take registers from this one.
 template <typename T, bool MASK, int THREADS, int H>
-__global__ __launch_bounds__(THREADS) void k_sample_long(SampleArgs g) {
+__global__ __launch_bounds__(THREADS) void k_sample_list(SampleArgs g) {
     using L = LongRow<T, MASK, THREADS, H>;
-    constexpr int N = Chunk<T>::N;
     __shared__ typename L::Shared sh;
     const int64_t row = blockIdx.x;
     const Settings s(g, row);
     L q(g, row, s, sh);
-    float top = -kInf;
-    int odd = 0;                                       // no distribution: a NaN or +inf
-    q.each_chunk([&](int, const float (&v)[N]) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            odd |= !(v[e] < kInf);
-            top = larger(v[e], top);
-        }
-    });
-    q.m = q.block_max(top);
-    const bool broken = __syncthreads_or(odd) != 0 || s.c != s.c;
-    if (broken || q.m == -kInf) {
-        if (threadIdx.x == 0) {
-            g.actions[row] = -1;
-            g.log_prob[row] = broken ? __builtin_nanf("") : 0.0f;
-        }
-        return;
-    }
-    Border b = everything();
+    float top;
+    double total;
+    if (!first_pass(q, g, row, top, total)) return;
     if (!s.all()) {
-        // the row's mass in 32 bits
-        float mass = 0.0f;
-        int allowed = 0;
-        const float c = s.c32();
-        q.bottom = -__FLT_MAX__;                       // not looked for: the window decides
-        q.each_chunk([&](int, const float (&v)[N]) {
-            float part = 0.0f;
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                part += __builtin_amdgcn_exp2f((v[e] - q.m) * c);
-                allowed += v[e] > -kInf;
-            }
-            mass += part;
-        });
-        const double total = q.block_sum((double)mass);
         const float bound = q.bound_of(top, (float)total);
         if (bound > -kInf) {
             const int n = q.gather_words([&](float v) { return v >= bound; });
@@ -1095,9 +1123,37 @@ __global__ __launch_bounds__(THREADS) void k_sample_long(SampleArgs g) {
                 return;
             }
         }
-        if (s.k > 0 || s.p < 1.0) b = border_of(q, s, q.m, s.p < 1.0 ? q.exact_mass() : total, q.block_sum(allowed));
     }
-    q.draw_from_row(g, row, b);
+    if (threadIdx.x == 0) g.actions[row] = kLeft;
+}
+
+// Whole rows: those that nothing cuts (CUT false: each of the launch), or those that the list left.
+template <typename T, bool MASK, int THREADS, int H, bool CUT>
+__global__ __launch_bounds__(THREADS) void k_sample_whole(SampleArgs g) {
+    using L = LongRow<T, MASK, THREADS, H>;
+    constexpr int N = L::N;
+    __shared__ typename L::Shared sh;
+    const int64_t row = blockIdx.x;
+    if (CUT && g.actions[row] != kLeft) return;
+    const Settings s(g, row);
+    L q(g, row, s, sh);
+    float top;
+    double total;
+    if (!first_pass(q, g, row, top, total)) return;
+    Border b = everything();
+    if (CUT && (s.k > 0 || s.p < 1.0)) {
+        int allowed = 0;
+        if (s.k > 0) {
+            q.each_chunk_again([&](int, const float (&v)[N]) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) allowed += v[e] > -kInf;
+            });
+            allowed = q.block_sum(allowed);
+        }
+        q.bottom = -__FLT_MAX__;                       // not looked for: the window decides
+        b = border_of(q, s, q.m, total, allowed);
+    }
+    q.template draw_from_row<CUT>(g, row, b);
 }
 
 __global__ void k_state_advance(unsigned long long* state) { state[1] += 1ull; }
@@ -1426,9 +1482,19 @@ void launch_sample(const SampleArgs& g, hipStream_t s) {
     }
     SHORT(4) SHORT(8) SHORT(16) SHORT(32) SHORT(64)
 #undef SHORT
-    if (chunks <= 256 * 4) hipLaunchKernelGGL((k_sample_long<T, MASK, 256, 4>), dim3((unsigned)g.rows), dim3(256), 0, s, g);
-    else if (chunks <= 1024 * 4) hipLaunchKernelGGL((k_sample_long<T, MASK, 1024, 4>), dim3((unsigned)g.rows), dim3(1024), 0, s, g);
-    else hipLaunchKernelGGL((k_sample_long<T, MASK, 1024, 16>), dim3((unsigned)g.rows), dim3(1024), 0, s, g);
+    const dim3 grid((unsigned)g.rows);
+    const bool all = !g.temperature && !g.top_k && !g.top_p && !g.min_p && g.temperature_s != 0.0f && g.top_k_s <= 0 && g.top_p_s >= 1.0f && !(g.min_p_s > 0.0f);
+#define LONG(THREADS, H)                                                                                                        \
+    if (all) {                                                                                                                  \
+        hipLaunchKernelGGL((k_sample_whole<T, MASK, THREADS, H, false>), grid, dim3(THREADS), 0, s, g);                         \
+    } else {                                                                                                                    \
+        hipLaunchKernelGGL((k_sample_list<T, MASK, THREADS, H>), grid, dim3(THREADS), 0, s, g);                                 \
+        hipLaunchKernelGGL((k_sample_whole<T, MASK, THREADS, 0, true>), grid, dim3(THREADS), 0, s, g);                          \
+    }
+    if (chunks <= 256 * 4) { LONG(256, 4) }
+    else if (chunks <= 1024 * 4) { LONG(1024, 4) }
+    else { LONG(1024, 16) }
+#undef LONG
 }
 
 template <typename T, bool MASK>

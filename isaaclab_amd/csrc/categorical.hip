@@ -1492,6 +1492,7 @@ void launch_sample(const SampleArgs& g, hipStream_t s) {
         hipLaunchKernelGGL((k_sample_whole<T, MASK, THREADS, 0, true>), grid, dim3(THREADS), 0, s, g);                          \
     }
     if (chunks <= 256 * 4) { LONG(256, 4) }
+    else if (chunks <= 256 * 16 && g.rows >= 512) { LONG(256, 16) }
     else if (chunks <= 1024 * 4) { LONG(1024, 4) }
     else { LONG(1024, 16) }
 #undef LONG

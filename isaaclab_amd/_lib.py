@@ -5,7 +5,6 @@ import fails loudly, and every wrapper raises if a tensor does not live on a HIP
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 import re
@@ -497,9 +496,15 @@ def stream(device=None):
 byref = C.byref
 
 
-def on_device(device: torch.device):
-    """Context in which ``device`` is the current one: a launch on its stream needs that."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # a tenth of what current_stream() takes
+
+
+def launch(fn, index: int, *args):
+    """``fn(*args, stream)`` with device ``index`` the current one, as a launch on its stream needs; errors as exceptions."""
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return launch(fn, index, *args)
+    check(fn(*args, _raw_stream(index) if _raw_stream is not None else stream(index)))
 
 
 def device_index(device) -> int:

@@ -73,6 +73,10 @@ def _per_row(t: torch.Tensor, name: str, dtype: torch.dtype, logits: torch.Tenso
     return t.contiguous()
 
 
+def _address(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
 _MOST = 3.4028234663852886e38
 
 
@@ -103,38 +107,34 @@ def sample_categorical(logits: torch.Tensor, u: torch.Tensor | None = None, *, t
         u = _per_row(u, "u", torch.float32, logits)
     else:
         state = M._state(logits.device)
-    actions = torch.empty(lead, dtype=torch.int64, device=logits.device)
-    log_prob = torch.empty(lead, dtype=torch.float32, device=logits.device)
+    actions, log_prob = x.new_empty(lead, dtype=torch.int64), x.new_empty(lead, dtype=torch.float32)
     a = L.MdpCategoricalSample(
-        x.data_ptr(), ld, x.shape[0], x.shape[1], L.DTYPES[x.dtype], 0, None if m is None else m.data_ptr(), ld_mask,
-        L.ptr(t_t), L.ptr(k_t), L.ptr(p_t), L.ptr(q_t), t_s, int(k_s), p_s, q_s, L.ptr(u), L.ptr(state),
+        x.data_ptr(), ld, x.shape[0], x.shape[1], L.DTYPES[x.dtype], 0, _address(m), ld_mask,
+        _address(t_t), _address(k_t), _address(p_t), _address(q_t), t_s, int(k_s), p_s, q_s, _address(u), _address(state),
         actions.data_ptr(), log_prob.data_ptr())
-    with L.on_device(logits.device):
-        L.check(L.lib.mdp_categorical_sample(L.byref(a), L.stream(logits.device)))
+    L.launch(L.lib.mdp_categorical_sample, x.get_device(), L.byref(a))
     return actions, log_prob
 
 
 def _eval_args(x, ld, actions, mask, ld_mask, t_t, t_s, log_prob, entropy, stats) -> "L.MdpCategoricalEval":
     return L.MdpCategoricalEval(x.data_ptr(), ld, x.shape[0], x.shape[1], L.DTYPES[x.dtype], t_s,
-                                None if mask is None else mask.data_ptr(), ld_mask, actions.data_ptr(), L.ptr(t_t),
-                                L.ptr(log_prob), L.ptr(entropy), L.ptr(stats))
+                                _address(mask), ld_mask, actions.data_ptr(), _address(t_t),
+                                _address(log_prob), _address(entropy), _address(stats))
 
 
 def _forward(x, ld, actions, mask, ld_mask, t_t, t_s, lead):
-    log_prob, entropy = (torch.empty(lead, dtype=torch.float32, device=x.device) for _ in range(2))
-    stats = torch.empty((x.shape[0], 3), dtype=torch.float32, device=x.device)
+    log_prob, entropy = x.new_empty(lead, dtype=torch.float32), x.new_empty(lead, dtype=torch.float32)
+    stats = x.new_empty((x.shape[0], 3), dtype=torch.float32)
     a = _eval_args(x, ld, actions, mask, ld_mask, t_t, t_s, log_prob, entropy, stats)
-    with L.on_device(x.device):
-        L.check(L.lib.mdp_categorical_evaluate(L.byref(a), L.stream(x.device)))
+    L.launch(L.lib.mdp_categorical_evaluate, x.get_device(), L.byref(a))
     return log_prob, entropy, stats
 
 
 def _backward(x, ld, actions, mask, ld_mask, t_t, t_s, stats, grad_log_prob, grad_entropy, shape):
-    grad = torch.empty(shape, dtype=x.dtype, device=x.device)
+    grad = x.new_empty(shape)
     a = _eval_args(x, ld, actions, mask, ld_mask, t_t, t_s, None, None, stats)
-    with L.on_device(x.device):
-        L.check(L.lib.mdp_categorical_evaluate_grad(L.byref(a), L.ptr(grad_log_prob), L.ptr(grad_entropy), grad.data_ptr(),
-                                                    x.shape[1], L.stream(x.device)))
+    L.launch(L.lib.mdp_categorical_evaluate_grad, x.get_device(), L.byref(a), _address(grad_log_prob), _address(grad_entropy),
+             grad.data_ptr(), x.shape[1])
     return grad
 
 

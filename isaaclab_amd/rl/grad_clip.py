@@ -88,16 +88,13 @@ def _launch(grads: list, outs: list | None, kind: int, max_norm: float | None) -
     if not grads:
         return torch.zeros((), dtype=torch.float32)
     table, index = _table(grads, outs)
-    n, device = len(grads), grads[0].device
-    workspace = torch.empty(L.lib.mdp_grad_workspace(n), dtype=torch.float64, device=device)
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    with L.on_device(device):
-        if max_norm is None:
-            rc = L.lib.mdp_grad_norm(table.buffer_info()[0], n, kind, workspace.data_ptr(), norm.data_ptr(), L.stream(index))
-        else:
-            rc = L.lib.mdp_grad_clip(table.buffer_info()[0], n, kind, max_norm, workspace.data_ptr(), norm.data_ptr(),
-                                     L.stream(index))
-    L.check(rc)
+    n, first = len(grads), grads[0]
+    workspace = first.new_empty(L.lib.mdp_grad_workspace(n), dtype=torch.float64)
+    norm = first.new_empty((), dtype=torch.float32)
+    if max_norm is None:
+        L.launch(L.lib.mdp_grad_norm, index, table.buffer_info()[0], n, kind, workspace.data_ptr(), norm.data_ptr())
+    else:
+        L.launch(L.lib.mdp_grad_clip, index, table.buffer_info()[0], n, kind, max_norm, workspace.data_ptr(), norm.data_ptr())
     return norm
 
 

@@ -642,13 +642,14 @@ struct LongRow {
     static constexpr int per_lane = 4;
     static constexpr float window = 24.0f;
     static constexpr bool total_known = false;
+    static constexpr double kLess = 1.0 - 1.53e-5, kMore = 1.0 + 1.53e-5;    // 2^-16: what the mass in 32 bits may be off
     struct Shared {
         double d[W + 1];
         int n[W + 1];
         float f[W];
         union {
             struct { float top[THREADS]; } maxima;
-            struct { uint64_t key[THREADS]; } list;
+            struct { uint64_t key[THREADS]; double value[THREADS]; } list;
         };
         uint32_t hist[per_lane * THREADS];
         Border border;
@@ -804,8 +805,8 @@ struct LongRow {
                 };
                 float lo = (float)((double)m - 60.0 / s.c), hi = m;
                 if (enough(lo)) {
-                    // twelve halvings: 60 binary orders of magnitude down to 1/64 of one, a few entries more than needed
-                    for (int it = 0; it < 12; ++it) {
+                    // ten halvings: 60 binary orders of magnitude down to 1/17 of one, a few entries more than needed
+                    for (int it = 0; it < 10; ++it) {
                         const float mid = 0.5f * lo + 0.5f * hi;
                         if (enough(mid)) lo = mid; else hi = mid;
                     }
@@ -823,40 +824,19 @@ struct LongRow {
         return sh.bound;
     }
 
-    // Gathers the entries that p names as words that sort by (value falling, place rising); their number, or -1 if there are too many.
-    template <class P>
-    MDP_DEV int gather_words(P&& p) const {
-        int mine = 0;
-        each_chunk([&](int, const float (&v)[N]) {
-#pragma unroll
-            for (int e = 0; e < N; ++e) mine += p(v[e]);
-        });
-        mine = group_sum<64>(mine);
+    // Lists the entries >= bound as words, in any order; their number, of which no more than THREADS are listed.
+    MDP_DEV int gather(float bound) const {
         __syncthreads();
-        if (lane == 0) sh.n[wave] = mine;
+        clear_list();
         __syncthreads();
-        int base = 0, total = 0;
-        for (int w = 0; w < W; ++w) {
-            if (w < wave) base += sh.n[w];
-            total += sh.n[w];
-        }
-        if (total > THREADS) return -1;
         each_chunk([&](int step, const float (&v)[N]) {
-            int n = 0;
+            const int i0 = place(wave, step);
 #pragma unroll
-            for (int e = 0; e < N; ++e) n += p(v[e]);
-            if (__any(n)) {
-                const int upto = group_scan<64>(n);
-                int to = base + upto - n;
-                const int i0 = place(wave, step);
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (p(v[e])) sh.list.key[to++] = word_of(v[e], i0 + e);
-                base += of_lane(upto, 63);
-            }
+            for (int e = 0; e < N; ++e)
+                if (v[e] >= bound) put<true>(v[e], i0 + e, 1.0);
         });
         __syncthreads();
-        return total;
+        return sh.listed;
     }
     template <class B, class F>
     MDP_DEV void sort_in(B&& bucket, F&& f) const {
@@ -918,21 +898,61 @@ struct LongRow {
     MDP_DEV uint64_t sort(uint64_t v, int n) const {
         int padded = 64;
         while (padded < n) padded <<= 1;
-        n = padded;
-        for (int size = 2; size < 2 * n; size <<= 1)
+        const bool works = tid < padded;               // waves beyond only keep the barriers
+        for (int size = 2; size < 2 * padded; size <<= 1)
             for (int stride = size >> 1; stride; stride >>= 1) {
-                uint64_t o;
-                if (stride < 64) o = __shfl_xor((unsigned long long)v, stride);
-                else {
+                if (stride >= 64) {
                     __syncthreads();
-                    sh.list.key[tid] = v;
+                    if (works) sh.list.key[tid] = v;
                     __syncthreads();
-                    o = sh.list.key[tid ^ stride];
                 }
+                if (!works) continue;
+                const uint64_t o = stride < 64 ? (uint64_t)__shfl_xor((unsigned long long)v, stride) : sh.list.key[tid ^ stride];
                 const bool low = !(tid & stride), rising = !(tid & size);
                 v = (o < v) == (low == rising) ? o : v;
             }
         return v;
+    }
+    MDP_DEV static int votes(bool v) { return __popcll(__ballot(v)); }
+    // how many of a wave's sorted entries are kept, by what `held` weighs; -1 if that is only the 32-bit mass and too near to tell
+    MDP_DEV int kept_of_few(int n, double ws, double before, double held, bool rough) const {
+        int kept = s.k > 0 ? min(s.k, n) : n;
+        if (s.p < 1.0) {
+            const int short_of = votes(lane < kept && before < s.p * held);
+            if (rough && (votes(lane < kept && before < s.p * held * kLess) != short_of || votes(lane < kept && before < s.p * held * kMore) != short_of)) return -1;
+            kept = min(kept, short_of);
+        }
+        return max(1, min(kept, votes(lane < n && ws >= s.mp)));
+    }
+    // the draw among n <= 64 candidates: the first wave's
+    MDP_DEV void draw_from_few(const SampleArgs& g, int64_t row, int n, double mass32) const {
+        uint64_t sorted = ~0ull;
+        double ws = 0.0, before = 0.0;
+        int kept = 1;
+        if (wave == 0) {
+            sorted = sort(lane < n ? sh.list.key[lane] : ~0ull, 64);
+            ws = lane < n ? s.weight(value_of(sorted), m) : 0.0;
+            const double upto = group_scan<64>(ws);
+            before = upto - ws;
+            kept = kept_of_few(n, ws, before, s.k > 0 ? of_lane(upto, min(s.k, n) - 1) : mass32, s.k == 0);
+            if (lane == 0) sh.found = kept;
+        }
+        if (s.p < 1.0 && s.k == 0) {
+            __syncthreads();
+            if (sh.found < 0) {
+                const double held = exact_mass();
+                if (wave == 0) kept = kept_of_few(n, ws, before, held, false);
+            }
+        }
+        if (wave) return;
+        const uint64_t by_place = sort(lane < kept ? sorted << 32 | (uint32_t)lane : ~0ull, 64);
+        const double from = __shfl(ws, (int)(uint32_t)by_place & 63);
+        const double kw = lane < kept ? from : 0.0;
+        const double line = group_scan<64>(kw), sum = of_lane(line, 63);
+        const double aim = s.u * sum;
+        const uint64_t over = __ballot(kw > 0.0 && line > aim), some = __ballot(kw > 0.0);
+        const int who = over ? __ffsll((unsigned long long)over) - 1 : 63 - __clzll((long long)some);
+        if (lane == who) answer(g, row, (int)(by_place >> 32), kw, sum);
     }
 
     MDP_DEV void answer(const SampleArgs& g, int64_t row, int i, double w, double mass) const {
@@ -940,10 +960,9 @@ struct LongRow {
         g.log_prob[row] = (float)log(w / mass);
     }
 
-    // the draw among n gathered candidates, among which is everything that k, p and min_p keep
+    // the draw among n listed candidates, among which is everything that k, p and min_p keep
     MDP_DEV void draw_from_list(const SampleArgs& g, int64_t row, int n, double mass32) const {
         const uint64_t word = tid < n ? sh.list.key[tid] : ~0ull;
-        const double w = tid < n ? s.weight(value_of(word), m) : 0.0;
         __syncthreads();
         const uint64_t sorted = sort(word, n);
         const double ws = tid < n ? s.weight(value_of(sorted), m) : 0.0;
@@ -955,9 +974,9 @@ struct LongRow {
             if (s.k > 0) held = block_sum(tid == kept - 1 ? upto : 0.0);
             int short_of = block_sum((int)(tid < kept && before < s.p * held));
             if (s.k == 0) {
-                // the row's mass in 32 bits decides unless the border is within its error (2^-16) of the aim
-                const int low = block_sum((int)(tid < kept && before < s.p * held * (1.0 - 1.53e-5)));
-                const int high = block_sum((int)(tid < kept && before < s.p * held * (1.0 + 1.53e-5)));
+                // the row's mass in 32 bits decides unless the border is within its error of the aim
+                const int low = block_sum((int)(tid < kept && before < s.p * held * kLess));
+                const int high = block_sum((int)(tid < kept && before < s.p * held * kMore));
                 if (low != high) {
                     held = exact_mass();
                     short_of = block_sum((int)(tid < kept && before < s.p * held));
@@ -967,12 +986,11 @@ struct LongRow {
         }
         kept = min(kept, block_sum((int)(tid < n && ws >= s.mp)));
         kept = max(kept, 1);
-        // the word of the last one that is kept tells by itself which entries of the list are
+        // those that are kept, by place
+        sh.list.value[tid] = ws;
         __syncthreads();
-        if (tid == kept - 1) sh.list.key[0] = sorted;
-        __syncthreads();
-        const uint64_t border = sh.list.key[0];
-        const double kw = tid < n && word <= border ? w : 0.0;
+        const uint64_t by_place = sort(tid < kept ? sorted << 32 | (uint32_t)tid : ~0ull, kept);
+        const double kw = tid < kept ? sh.list.value[(uint32_t)by_place] : 0.0;
         double sum;
         const double line = block_scan(kw, sum);
         const double aim = s.u * sum;
@@ -984,7 +1002,7 @@ struct LongRow {
         }
         __syncthreads();
         const int who = sh.found < THREADS ? sh.found : sh.last;
-        if (tid == who) answer(g, row, (int)(uint32_t)word, kw, sum);
+        if (tid == who) answer(g, row, (int)(by_place >> 32), kw, sum);
     }
 
     MDP_DEV double kept_mass(const Border& b, const float (&v)[N], int i0, double (&w)[N]) const {
@@ -1117,9 +1135,10 @@ __global__ __launch_bounds__(THREADS) void k_sample_list(SampleArgs g) {
     if (!s.all()) {
         const float bound = q.bound_of(top, (float)total);
         if (bound > -kInf) {
-            const int n = q.gather_words([&](float v) { return v >= bound; });
-            if (n > 0) {
-                q.draw_from_list(g, row, n, total);
+            const int n = q.gather(bound);
+            if (n <= THREADS) {
+                if (n <= 64) q.draw_from_few(g, row, n, total);
+                else q.draw_from_list(g, row, n, total);
                 return;
             }
         }

@@ -194,6 +194,7 @@ struct SampleArgs {
     const void* logits; int64_t ld;
     const uint8_t* mask; int64_t ld_mask;
     int vocab; int64_t rows;
+    int64_t row0;                                      // of the call's rows the launch's first
     const float* temperature; const int* top_k; const float* top_p; const float* min_p;
     float temperature_s; int top_k_s; float top_p_s; float min_p_s;
     const float* u; const unsigned long long* state;
@@ -202,7 +203,8 @@ struct SampleArgs {
 
 constexpr uint32_t kStream = 0x43415447u;
 
-// A row's settings.  Temperature 0 is one entry of the largest logit, with weights that are 1 there and 0 elsewhere.
+// A row's settings.  Temperature 0 (and what is below the smallest normal number) is one entry of the largest logit, with weights
+// that are 1 there and 0 elsewhere.
 struct Settings {
     double c;                                          // log2(e) / T; a NaN for a temperature that is negative or NaN
     int k;                                             // 0: no limit
@@ -217,12 +219,12 @@ struct Settings {
         mp = mf > 0.0f ? (mf < 1.0f ? (double)mf : 1.0) : 0.0;
         c = 1.4426950408889634 / (double)t;
         c = c > 1e-300 ? c : 1e-300;                   // infinite temperature: -inf * c stays -inf
-        if (t == 0.0f) { c = 1e300; k = 1; p = 1.0; mp = 0.0; }
+        if (t >= 0.0f && t < 1.17549435e-38f) { c = 1e300; k = 1; p = 1.0; mp = 0.0; }
         if (!(t >= 0.0f)) c = __builtin_nan("");
-        float uf = g.u ? g.u[row] : u01(rng4(g.state[0], g.state[1], kStream, (uint64_t)row).x);
+        float uf = g.u ? g.u[row] : u01(rng4(g.state[0], g.state[1], kStream, (uint64_t)(g.row0 + row)).x);
         u = uf > 0.0f ? (uf < 0.99999994f ? (double)uf : 0.99999994039535522) : 0.0;
     }
-    MDP_DEV float c32() const { return (float)fmax(fmin(c, 1e30), 1e-30); }     // -inf * c and 0 * c stay what they are
+    MDP_DEV float c32() const { return (float)fmax(fmin(c, 3e38), 1e-38); }     // -inf * c and 0 * c stay what they are
     MDP_DEV bool all() const { return k == 0 && p == 1.0 && mp == 0.0; }
     MDP_DEV double weight(float x, float m) const { return exp2_neg(((double)x - (double)m) * c); }
 };
@@ -1093,13 +1095,13 @@ MDP_DEV bool first_pass(L& q, const SampleArgs& g, int64_t row, float& top, doub
     constexpr int N = L::N;
     const float c = q.s.c32();
     top = -__FLT_MAX__;
-    float part = 0.0f;
+    double part = 0.0;                                 // sums of chunks: a long row has many
     q.each_chunk([&](int, const float (&v)[N]) {
         float to = top;
 #pragma unroll
         for (int e = 0; e < N; ++e) to = larger(v[e], to);
         if (to > top) {
-            part *= __builtin_amdgcn_exp2f(larger((top - to) * c, -300.0f));
+            part *= (double)__builtin_amdgcn_exp2f(larger((top - to) * c, -300.0f));
             top = to;
         }
         float sum = 0.0f;
@@ -1108,7 +1110,7 @@ MDP_DEV bool first_pass(L& q, const SampleArgs& g, int64_t row, float& top, doub
         part += sum;
     });
     q.m = q.block_max(top);
-    total = q.block_sum((double)(part * __builtin_amdgcn_exp2f(larger((top - q.m) * c, -300.0f))));
+    total = q.block_sum(part * (double)__builtin_amdgcn_exp2f(larger((top - q.m) * c, -300.0f)));
     const bool broken = total != total || q.s.c != q.s.c;
     if (total > 0.0 && !broken) return true;
     if (threadIdx.x == 0) {
@@ -1213,13 +1215,14 @@ MDP_DEV float inverse_temperature(const float* per_row, float scalar, int64_t ro
 }
 
 struct Running {
-    float m, s, t;
-    MDP_DEV static Running none() { return Running{-__FLT_MAX__, 0.0f, 0.0f}; }
+    float m;
+    double s, t;                                       // of chunks that were summed up in 32 bits
+    MDP_DEV static Running none() { return Running{-__FLT_MAX__, 0.0, 0.0}; }
     MDP_DEV void move(float to, float c) {             // about another maximum >= m
         float d = (m - to) * c;
         d = d < -300.0f ? -300.0f : d;                 // 2^-300 is 0: 0 * inf must not arise
-        const float f = __builtin_amdgcn_exp2f(d);
-        t = f * (t + d * s);
+        const double f = (double)__builtin_amdgcn_exp2f(d);
+        t = f * (t + (double)d * s);
         s *= f;
         m = to;
     }
@@ -1239,14 +1242,14 @@ struct Running {
 };
 
 template <typename T>
-MDP_DEV void finish_row(const EvalArgs& g, const Row<T>& r, int64_t row, float m, float s, float t, float inv_t) {
-    const float log_s = logf(s);
-    const float h = s == 0.0f ? 0.0f : log_s - kLn2 * (t / s);
+MDP_DEV void finish_row(const EvalArgs& g, const Row<T>& r, int64_t row, float m, double s, double t, float inv_t) {
+    const float log_s = logf((float)s);
+    const float h = s == 0.0 ? 0.0f : log_s - kLn2 * (float)(t / s);
     const int64_t a = g.actions[row];
     float lp;
     if (a == -1) lp = 0.0f;
     else if (a < 0 || a >= r.V) lp = __builtin_nanf("");
-    else if (!r.allowed((int)a)) lp = s == s ? -kInf : s;
+    else if (!r.allowed((int)a)) lp = s == s ? -kInf : (float)s;
     else lp = (to_f32(r.x[a]) - m) * inv_t - log_s;
     g.log_prob[row] = lp;
     g.entropy[row] = h;
@@ -1286,7 +1289,8 @@ __global__ __launch_bounds__(256) void k_evaluate_short(EvalArgs g) {
 template <typename T, bool MASK>
 __global__ __launch_bounds__(256) void k_evaluate_long(EvalArgs g) {
     constexpr int N = Chunk<T>::N, B = 4;
-    __shared__ float wave_m[4], wave_s[4], wave_t[4];
+    __shared__ float wave_m[4];
+    __shared__ double wave_s[4], wave_t[4];
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x;
     const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
@@ -1472,12 +1476,13 @@ int check_rows(const char* what, const void* logits, int64_t rows, int64_t vocab
                int64_t ld_mask) {
     MDP_REQUIRE(rows >= 0 && vocab >= 0, "%s: negative shape (%lld, %lld)", what, (long long)rows, (long long)vocab);
     MDP_REQUIRE(dtype >= 0 && dtype < MDP_DTYPE_NUM, "%s: unknown element type %d", what, dtype);
-    MDP_REQUIRE(rows <= 0x7fffffff, "%s: %lld rows are beyond one launch", what, (long long)rows);
+    MDP_REQUIRE(rows <= ((int64_t)1 << 40), "%s: %lld rows are too many", what, (long long)rows);
     MDP_REQUIRE(vocab < (1 << 30), "%s: rows of %lld entries are too long", what, (long long)vocab);
     if (rows == 0) return MDP_OK;
     MDP_REQUIRE(vocab > 0, "%s: rows without entries", what);
     MDP_REQUIRE(logits, "%s: null logits", what);
     MDP_REQUIRE(ld >= 0 && ld_mask >= 0, "%s: negative row stride", what);
+    MDP_REQUIRE((uintptr_t)logits % (dtype == MDP_DTYPE_F32 ? 4 : 2) == 0, "%s: logits between two elements", what);
     return MDP_OK;
 }
 
@@ -1502,7 +1507,7 @@ void launch_sample(const SampleArgs& g, hipStream_t s) {
     SHORT(4) SHORT(8) SHORT(16) SHORT(32) SHORT(64)
 #undef SHORT
     const dim3 grid((unsigned)g.rows);
-    const bool all = !g.temperature && !g.top_k && !g.top_p && !g.min_p && g.temperature_s != 0.0f && g.top_k_s <= 0 && g.top_p_s >= 1.0f && !(g.min_p_s > 0.0f);
+    const bool all = !g.temperature && !g.top_k && !g.top_p && !g.min_p && g.temperature_s >= 1.17549435e-38f && g.top_k_s <= 0 && g.top_p_s >= 1.0f && !(g.min_p_s > 0.0f);
 #define LONG(THREADS, H)                                                                                                        \
     if (all) {                                                                                                                  \
         hipLaunchKernelGGL((k_sample_whole<T, MASK, THREADS, H, false>), grid, dim3(THREADS), 0, s, g);                         \
@@ -1540,10 +1545,19 @@ void launch_grad(GradArgs g, hipStream_t s) {
     }
     SHORT(4, 1) SHORT(4, 2) SHORT(4, 4) SHORT(8, 4) SHORT(16, 4) SHORT(32, 4) SHORT(64, 4)
 #undef SHORT
-    const int64_t most = 0x7fffffff / g.rows;          // a launch's blocks
+    const int64_t most = ((1 << 24) - 1) / g.rows;     // a launch's blocks of 256 threads
     g.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(most, (chunks + 1023) / 1024));
     hipLaunchKernelGGL((k_grad_long<T, MASK>), dim3((unsigned)(g.rows * g.pieces)), dim3(256), 0, s, g);
 }
+
+// A launch holds fewer than 2^32 threads: calls of more rows than blocks of 1024 fill that with are cut, f(first row, rows).
+constexpr int64_t kRows = 1 << 21;
+template <class F>
+void by_rows(int64_t rows, F&& f) {
+    for (int64_t at = 0; at < rows; at += kRows) f(at, std::min(kRows, rows - at));
+}
+template <typename P>
+P* offset(P* p, int64_t by) { return p ? p + by : p; }
 
 template <class F>
 void by_type(int dtype, bool mask, F&& f) {
@@ -1560,11 +1574,17 @@ extern "C" int mdp_categorical_sample(const mdp_categorical_sample_t* a, void* s
     if (a->rows == 0) return MDP_OK;
     MDP_REQUIRE(a->actions && a->log_prob, "categorical_sample: null output");
     MDP_REQUIRE(a->u || a->state, "categorical_sample needs uniforms or a generator state {seed, epoch}");
-    SampleArgs g{a->logits, a->ld, a->mask, a->ld_mask, (int)a->vocab, a->rows, a->temperature, a->top_k, a->top_p, a->min_p,
-                 a->temperature_scalar, a->top_k_scalar, a->top_p_scalar, a->min_p_scalar, a->u,
-                 (const unsigned long long*)a->state, a->actions, a->log_prob};
     hipStream_t s = as_stream(stream);
-    by_type(a->dtype, a->mask, [&](auto t, auto m) { launch_sample<decltype(t), decltype(m)::value>(g, s); });
+    by_type(a->dtype, a->mask, [&](auto t, auto m) {
+        using T = decltype(t);
+        by_rows(a->rows, [&](int64_t at, int64_t rows) {
+            const SampleArgs g{(const T*)a->logits + at * a->ld, a->ld, offset(a->mask, at * a->ld_mask), a->ld_mask, (int)a->vocab,
+                               rows, at, offset(a->temperature, at), offset(a->top_k, at), offset(a->top_p, at), offset(a->min_p, at),
+                               a->temperature_scalar, a->top_k_scalar, a->top_p_scalar, a->min_p_scalar, offset(a->u, at),
+                               (const unsigned long long*)a->state, a->actions + at, a->log_prob + at};
+            launch_sample<T, decltype(m)::value>(g, s);
+        });
+    });
     if (!a->u) hipLaunchKernelGGL(k_state_advance, dim3(1), dim3(1), 0, s, (unsigned long long*)a->state);
     MDP_LAUNCH_CHECK();
     return MDP_OK;
@@ -1575,10 +1595,16 @@ extern "C" int mdp_categorical_evaluate(const mdp_categorical_eval_t* a, void* s
     if (int rc = check_rows("categorical_evaluate", a->logits, a->rows, a->vocab, a->ld, a->dtype, a->mask, a->ld_mask)) return rc;
     if (a->rows == 0) return MDP_OK;
     MDP_REQUIRE(a->actions && a->log_prob && a->entropy, "categorical_evaluate: null pointer");
-    EvalArgs g{a->logits, a->ld, a->mask, a->ld_mask, (int)a->vocab, a->rows, a->actions, a->temperature, a->temperature_scalar,
-               a->log_prob, a->entropy, a->stats};
     hipStream_t s = as_stream(stream);
-    by_type(a->dtype, a->mask, [&](auto t, auto m) { launch_evaluate<decltype(t), decltype(m)::value>(g, s); });
+    by_type(a->dtype, a->mask, [&](auto t, auto m) {
+        using T = decltype(t);
+        by_rows(a->rows, [&](int64_t at, int64_t rows) {
+            const EvalArgs g{(const T*)a->logits + at * a->ld, a->ld, offset(a->mask, at * a->ld_mask), a->ld_mask, (int)a->vocab, rows,
+                             a->actions + at, offset(a->temperature, at), a->temperature_scalar, a->log_prob + at, a->entropy + at,
+                             offset(a->stats, 3 * at)};
+            launch_evaluate<T, decltype(m)::value>(g, s);
+        });
+    });
     MDP_LAUNCH_CHECK();
     return MDP_OK;
 }
@@ -1590,10 +1616,17 @@ extern "C" int mdp_categorical_evaluate_grad(const mdp_categorical_eval_t* a, co
     if (a->rows == 0) return MDP_OK;
     MDP_REQUIRE(a->actions && a->stats && grad_logits, "categorical_evaluate_grad: null pointer");
     MDP_REQUIRE(ld_grad >= a->vocab, "categorical_evaluate_grad: gradient rows overlap");
-    GradArgs g{a->logits, a->ld, a->mask, a->ld_mask, (int)a->vocab, a->rows, a->actions, a->temperature, a->temperature_scalar,
-               a->stats, grad_log_prob, grad_entropy, grad_logits, ld_grad, 1};
+    MDP_REQUIRE((uintptr_t)grad_logits % (a->dtype == MDP_DTYPE_F32 ? 4 : 2) == 0, "categorical_evaluate_grad: gradient between two elements");
     hipStream_t s = as_stream(stream);
-    by_type(a->dtype, a->mask, [&](auto t, auto m) { launch_grad<decltype(t), decltype(m)::value>(g, s); });
+    by_type(a->dtype, a->mask, [&](auto t, auto m) {
+        using T = decltype(t);
+        by_rows(a->rows, [&](int64_t at, int64_t rows) {
+            const GradArgs g{(const T*)a->logits + at * a->ld, a->ld, offset(a->mask, at * a->ld_mask), a->ld_mask, (int)a->vocab, rows,
+                             a->actions + at, offset(a->temperature, at), a->temperature_scalar, a->stats + 3 * at,
+                             offset(grad_log_prob, at), offset(grad_entropy, at), (T*)grad_logits + at * ld_grad, ld_grad, 1};
+            launch_grad<T, decltype(m)::value>(g, s);
+        });
+    });
     MDP_LAUNCH_CHECK();
     return MDP_OK;
 }

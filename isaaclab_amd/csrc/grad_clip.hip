@@ -209,10 +209,12 @@ int check_grads(const mdp_grad_t* g, int64_t n, int kind, const double* workspac
         MDP_REQUIRE(g[i].count <= kMost && (total += g[i].count) <= kMost, "grad norm: more than 2^40 elements");
         MDP_REQUIRE(g[i].dtype >= 0 && g[i].dtype < MDP_DTYPE_NUM, "grad norm: tensor %lld has element type %d", (long long)i, g[i].dtype);
         MDP_REQUIRE(!g[i].count || g[i].grad, "grad norm: tensor %lld is null", (long long)i);
+        MDP_REQUIRE((uintptr_t)g[i].grad % bytes_of(g[i].dtype) == 0, "grad norm: tensor %lld starts between two elements", (long long)i);
         if (!clip) continue;
         MDP_REQUIRE(!g[i].count || g[i].out, "grad_clip: output %lld is null", (long long)i);
         MDP_REQUIRE(g[i].out_dtype == g[i].dtype || g[i].out_dtype == MDP_DTYPE_F32,
                     "grad_clip: output %lld is neither of its gradient's type nor float32", (long long)i);
+        MDP_REQUIRE((uintptr_t)g[i].out % bytes_of(g[i].out_dtype) == 0, "grad_clip: output %lld starts between two elements", (long long)i);
     }
     return MDP_OK;
 }

@@ -56,6 +56,8 @@ def _setting(value, name: str, dtype: torch.dtype, logits: torch.Tensor, low: fl
         return None, value
     if value.device != logits.device:
         raise ValueError(f"{name} lives on '{value.device}', logits on '{logits.device}'")
+    if value.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} gets no gradient: pass it detached")
     lead = logits.shape[:-1]
     if dtype == torch.int32 and value.dtype != dtype:
         value = value.clamp(-1, 2147483647)
@@ -90,11 +92,12 @@ def sample_categorical(logits: torch.Tensor, u: torch.Tensor | None = None, *, t
 
     Kept are the ``top_k`` largest allowed logits (0: all; equal ones by lowest index), of these the fewest largest that hold a
     share ``top_p`` of their weight (one at least), of these the ones of at least ``min_p`` times the largest weight.
-    ``temperature`` 0 takes the largest logit (the first of equal ones) with log_prob 0.  ``log_prob`` is that of the
+    ``temperature`` 0 (or below the smallest normal float) takes the largest logit (the first of equal ones) with log_prob 0.  ``log_prob`` is that of the
     distribution drawn from: without ``top_k`` / ``top_p`` / ``min_p`` it is what ``evaluate_categorical`` says.
 
     A row in which nothing is allowed gives action -1 and log_prob 0; a row with a NaN or +inf among its allowed logits gives
-    action -1 and log_prob NaN, and so does a per-row temperature that is negative or NaN.  No gradient."""
+    action -1 and log_prob NaN, and so does a per-row temperature that is negative or NaN.  A per-row ``top_p`` / ``min_p`` that is
+    NaN sets no limit.  No gradient."""
     x, ld = _logit_rows(logits)
     m, ld_mask = _mask_rows(mask, logits)
     lead = logits.shape[:-1]
@@ -182,6 +185,8 @@ def evaluate_categorical(logits: torch.Tensor, actions: torch.Tensor, *, tempera
     Inside a captured graph use ``evaluate_categorical_grad``, which does without autograd's own streams and graph nodes."""
     L.require_gpu(logits, "logits")
     actions = _per_row(actions, "actions", torch.int64, logits)
+    if isinstance(temperature, torch.Tensor) and temperature.requires_grad and torch.is_grad_enabled():
+        raise ValueError("temperature gets no gradient: pass it detached")
     return _Evaluate.apply(logits, actions, mask, temperature)
 
 

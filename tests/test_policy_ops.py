@@ -89,8 +89,10 @@ def test_refusals_before_any_launch():
     assert L.lib.mdp_categorical_sample(C.byref(a), None) == L.MDP_ERR_INVALID and "null output" in L.last_error()
     a.actions = a.log_prob = 4096
     assert L.lib.mdp_categorical_sample(C.byref(a), None) == L.MDP_ERR_INVALID and "generator state" in L.last_error()
-    a.rows = 1 << 40
-    assert L.lib.mdp_categorical_sample(C.byref(a), None) == L.MDP_ERR_INVALID and "beyond one launch" in L.last_error()
+    a.rows = 1 << 41
+    assert L.lib.mdp_categorical_sample(C.byref(a), None) == L.MDP_ERR_INVALID and "too many" in L.last_error()
+    a.rows, a.logits = 2, 4098
+    assert L.lib.mdp_categorical_sample(C.byref(a), None) == L.MDP_ERR_INVALID and "between two elements" in L.last_error()
     a.rows = 0
     assert L.lib.mdp_categorical_sample(C.byref(a), None) == L.MDP_OK
     e = L.MdpCategoricalEval()
@@ -114,7 +116,7 @@ def test_refusals_before_any_launch():
                      ([ok, (8192, 4096 + 60, 4, 0, 0)], {}),                     # an output inside another gradient
                      ([(8192, 4096, 16, 0, 0), (16384, 4096 + 32, 2, 0, 0)], {}),   # two outputs overlap
                      ([(4096, 4100, 16, 0, 0)], {}),                             # an output shifted over its own gradient
-                     ([(4096, 4096, 1 << 41, 0, 0)], {})]:
+                     ([(4096, 4096, 1 << 41, 0, 0)], {}), ([(4098, 4098, 4, 0, 0)], {}), ([(4096, 8193, 4, 1, 1)], {})]:
         assert clip(rows, **kw) == L.MDP_ERR_INVALID, (rows, kw)
         assert L.last_error()
     assert L.lib.mdp_grad_norm(None, 1, 2, 64, 64, None) == L.MDP_ERR_INVALID
@@ -497,6 +499,7 @@ def test_evaluation_layouts_and_autograd(device):
     for match, call in [("actions must be", lambda: rl.evaluate_categorical(base, a.int())),
                         ("actions must be", lambda: rl.evaluate_categorical(base, a[:2])),
                         ("temperature", lambda: rl.evaluate_categorical(base, a, temperature=0.0)),
+                        ("no gradient", lambda: rl.evaluate_categorical(base, a, temperature=t.clone().requires_grad_())),
                         ("grad_entropy", lambda: rl.evaluate_categorical_grad(base, a, None, one.double()))]:
         with pytest.raises(ValueError, match=match):
             call()
@@ -518,6 +521,64 @@ def test_offsets_beyond_32_bits(device):
     one = torch.ones(rows, device=device)
     lp, h, grad = rl.evaluate_categorical_grad(x, a, one, one)
     check_evaluation(last, a[-1:], lp[-1:], h[-1:], grad[-1:], one[:1], one[:1])
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_holds(device):
+    """Rows beyond 2^21 are drawn, evaluated and differentiated by further launches; the generator goes by the row of the call."""
+    from isaaclab_amd.utils import math as M
+
+    rows, n = (1 << 21) + 1003, 5
+    g = torch.Generator(device=device).manual_seed(3)
+    x = torch.randn(rows, 3, generator=g, device=device)
+    u = torch.rand(rows, generator=g, device=device)
+    temperature = torch.rand(rows, generator=g, device=device) + 0.5
+    mask = torch.rand(rows, 3, generator=g, device=device) < 0.8
+    got = rl.sample_categorical(x, u, mask=mask, top_p=0.8, temperature=temperature)
+    gl = torch.randn(rows, generator=g, device=device)
+    lp, h, grad = rl.evaluate_categorical_grad(x, got[0], gl, gl, mask=mask, temperature=temperature)
+    for at in (0, (1 << 21) - n, 1 << 21, rows - n):
+        part = slice(at, at + n)
+        check_draw(x[part], u[part], (got[0][part], got[1][part]), mask=mask[part], top_p=0.8, temperature=temperature[part])
+        check_evaluation(x[part], got[0][part], lp[part], h[part], grad[part], gl[part], gl[part], mask=mask[part],
+                         temperature=temperature[part])
+    M.seed_samplers(4, device)
+    a = rl.sample_categorical(x[:1].expand(rows, 3))[0]
+    assert not torch.equal(a[:1003], a[1 << 21:])
+    M.seed_samplers(1, device)
+
+
+@pytest.mark.gpu
+def test_a_very_long_row(device):
+    """Sums of many more terms than 24 bits count: a flat row of 3.3e7 entries."""
+    vocab = (1 << 25) + 77
+    x = torch.zeros(1, vocab, dtype=torch.float16, device=device)
+    u = torch.tensor([0.75], device=device)
+    a, lp = rl.sample_categorical(x, u)
+    assert a.item() == int(0.75 * vocab)                            # the first i with i + 1 > 0.75 vocab
+    np.testing.assert_allclose(lp.item(), -math.log(vocab), rtol=2 * U)
+    a, lp = rl.sample_categorical(x, u, top_p=0.5)
+    kept = math.ceil(0.5 * vocab)
+    assert a.item() == int(0.75 * kept)
+    np.testing.assert_allclose(lp.item(), -math.log(kept), rtol=2 * U)
+    one = torch.ones(1, device=device)
+    lp, h, grad = rl.evaluate_categorical_grad(x, a, one, one)
+    # exact sums: what is left is the rounding of ln s and of one product
+    np.testing.assert_allclose([lp.item(), h.item()], [-math.log(vocab), math.log(vocab)], rtol=4 * U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [9, 3000])
+def test_smallest_temperatures(device, vocab):
+    """Down to the smallest normal number the definition holds -- logits that lie 1e-37 apart are then far apart --, below it the
+    largest logit is taken."""
+    g = rng_of("cold", vocab)
+    x = (torch.rand(6, vocab, generator=g) * 4e-36).to(device)
+    u = torch.rand(6, generator=g).to(device)
+    t = torch.tensor([2e-36, 1.2e-38, 1e-39, 1e-45, 1e-30, 3e38], device=device)
+    a, lp = rl.sample_categorical(x, u, temperature=t, top_p=0.9)
+    exact = torch.where(t < 1.1754944e-38, 0.0, t)
+    check_draw(x, u, (a, lp), temperature=exact, top_p=0.9)
 
 
 # -- gradients --------------------------------------------------------------------------------------------------------

@@ -323,7 +323,7 @@ void launch_evaluate(const EvalArgs& g, hipStream_t s) {
         hipLaunchKernelGGL((k_evaluate_short<T, MASK, G, K>), dim3((unsigned)((g.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, s, g); \
         return;                                                                                                                \
     }
-    SHORT(4, 1) SHORT(4, 2) SHORT(4, 4) SHORT(8, 4) SHORT(16, 4) SHORT(32, 4) SHORT(64, 4)
+    SHORT(4, 1) SHORT(4, 2) SHORT(4, 4) SHORT(8, 4) SHORT(16, 4) SHORT(32, 4) SHORT(64, 4) SHORT(64, 8)
 #undef SHORT
     hipLaunchKernelGGL((k_evaluate_long<T, MASK>), dim3((unsigned)g.rows), dim3(256), 0, s, g);
 }
@@ -336,7 +336,7 @@ void launch_grad(GradArgs g, hipStream_t s) {
         hipLaunchKernelGGL((k_grad_short<T, MASK, G, K>), dim3((unsigned)((g.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, s, g); \
         return;                                                                                                            \
     }
-    SHORT(4, 1) SHORT(4, 2) SHORT(4, 4) SHORT(8, 4) SHORT(16, 4) SHORT(32, 4) SHORT(64, 4)
+    SHORT(4, 1) SHORT(4, 2) SHORT(4, 4) SHORT(8, 4) SHORT(16, 4) SHORT(32, 4) SHORT(64, 4) SHORT(64, 8)
 #undef SHORT
     const int64_t most = ((1 << 24) - 1) / g.rows;     // a launch's blocks of 256 threads
     g.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(most, (chunks + 1023) / 1024));

@@ -212,16 +212,17 @@ MDP_DEV void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Rows of up to G K chunks, 16 entries a lane: G lanes of a wave hold a row and its weights in registers.  Groups of a wave go
-// through their loops together until the last is done.
+// Rows of up to G K chunks, 16 entries a lane: G lanes of a wave, or a block of G = 128 or 256, hold a row and its weights in
+// registers.  Groups of a wave go through their loops together until the last is done.
 template <typename T, int G, int K>
 struct ShortRow {
     static constexpr int N = Chunk<T>::N, size = G, capacity = G;
-    static constexpr int per_lane = G < 8 ? 16 : G < 32 ? 8 : 4;
+    static constexpr int per_lane = G < 8 ? 16 : G < 32 ? 8 : G <= 64 ? 4 : 256 / G;      // at most 256 buckets: their numbers are bytes
+    static constexpr int W = G / 64;                   // waves of a block that holds one row
     static constexpr float window = 14.0f;
     static constexpr bool total_known = true;
     struct Listed { uint64_t word; double value; };      // the word rises in the order
-    struct Shared { Listed list[G]; uint32_t hist[per_lane * G]; int n; };
+    struct Shared { Listed list[G]; double d[W ? W : 1]; uint32_t u[W ? W : 1]; uint32_t hist[per_lane * G]; int n; };
     float x[K][N];
     double w[K][N];
     int rank, shift;                                   // this lane's number; the row's shift
@@ -242,12 +243,72 @@ struct ShortRow {
             for (int e = 0; e < N; ++e) f(x[k][e], base + k * G * N + e, [&] { return w[k][e]; });
     }
     MDP_DEV double weight(float v) const { return s->weight(v, m); }
-    template <typename V> MDP_DEV V sum(V v) const { return group_sum<G>(v); }
-    MDP_DEV float highest(float v) const { return group_max<G>(v); }
-    MDP_DEV float lowest(float v) const { return -group_max<G>(-v); }
-    template <typename V> MDP_DEV V scan(V v) const { return group_scan<G>(v); }
-    MDP_DEV void sync() const { wave_sync(); }
-    MDP_DEV bool any(bool v) const { return __any(v && good) != 0; }
+    // the waves' values, for a block
+    template <typename V, class F>
+    MDP_DEV void exchange(V v, bool mine, F&& f) const {
+        const int wave = threadIdx.x >> 6;
+        __syncthreads();
+        if (mine) {
+            if constexpr (sizeof(V) == 8) sh->d[wave] = v;
+            else sh->u[wave] = __builtin_bit_cast(uint32_t, v);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if constexpr (sizeof(V) == 8) f(i, sh->d[i]);
+            else f(i, __builtin_bit_cast(V, sh->u[i]));
+        }
+    }
+    template <typename V>
+    MDP_DEV V sum(V v) const {
+        if constexpr (G <= 64) return group_sum<G>(v);
+        V all = V(0);
+        exchange(group_sum<64>(v), (threadIdx.x & 63) == 0, [&](int, V o) { all += o; });
+        return all;
+    }
+    MDP_DEV float highest(float v) const {
+        if constexpr (G <= 64) return group_max<G>(v);
+        float all = -kInf;
+        exchange(group_max<64>(v), (threadIdx.x & 63) == 0, [&](int, float o) { all = larger(o, all); });
+        return all;
+    }
+    MDP_DEV float lowest(float v) const { return -highest(-v); }
+    template <typename V>
+    MDP_DEV V scan(V v) const {
+        if constexpr (G <= 64) return group_scan<G>(v);
+        v = group_scan<64>(v);
+        V before = V(0);
+        exchange(v, (threadIdx.x & 63) == 63, [&](int i, V o) { before += i < (int)(threadIdx.x >> 6) ? o : V(0); });
+        return before + v;
+    }
+    // the votes of a group that is not a block, from its first lane on
+    MDP_DEV uint64_t votes(bool v) const {
+        const uint64_t all = __ballot(v) >> ((threadIdx.x & 63) - rank);
+        return G == 64 ? all : all & ((1ull << (G & 63)) - 1ull);
+    }
+    // the group's first (last) lane of which v holds, -1 if none
+    MDP_DEV int first_of(bool v) const {
+        if constexpr (G <= 64) return __ffsll((unsigned long long)votes(v)) - 1;
+        const int at = (int)lowest(v ? (float)rank : (float)G);
+        return at < G ? at : -1;
+    }
+    MDP_DEV int last_of(bool v) const {
+        if constexpr (G <= 64) return 63 - __clzll((long long)votes(v));
+        return (int)highest(v ? (float)rank : -1.0f);
+    }
+    MDP_DEV bool some(bool v) const {
+        if constexpr (G <= 64) return votes(v) != 0;
+        else return __syncthreads_or(v) != 0;
+    }
+    MDP_DEV void sync() const {
+        if constexpr (G <= 64) wave_sync();
+        else __syncthreads();
+    }
+    // over the lanes that run a loop in step: a wave's groups; a block's lanes all say the same
+    MDP_DEV bool any(bool v) const {
+        if constexpr (G <= 64) return __any(v && good) != 0;
+        else return v && good;
+    }
     // the buckets of the entries, a byte each
     uint32_t ids[4];
     template <class B, class F>
@@ -289,7 +350,7 @@ struct ShortRow {
         const uint64_t mine = in ? sh->list[rank].word : ~0ull;
         double before = above;
         int order = 0;
-        for (int j = 0; __any(j < n); ++j) {
+        for (int j = 0; G <= 64 ? __any(j < n) != 0 : j < n; ++j) {
             const Listed o = sh->list[j];              // beyond n: what was there before
             const bool first = j < n && o.word < mine;
             before += first ? o.value : 0.0;
@@ -321,14 +382,13 @@ struct ShortRow {
 };
 
 template <typename T, bool MASK, int G, int K>
-__global__ __launch_bounds__(256, 4) void k_sample_short(SampleArgs g) {
+__global__ __launch_bounds__(G > 64 ? G : 256, 4) void k_sample_short(SampleArgs g) {
     using R = ShortRow<T, G, K>;
-    constexpr int N = Chunk<T>::N;
-    __shared__ typename R::Shared shared[256 / G];
-    const int64_t mine = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    constexpr int N = Chunk<T>::N, ROWS = G > 64 ? 1 : 256 / G;
+    __shared__ typename R::Shared shared[ROWS];
+    const int64_t mine = (int64_t)blockIdx.x * ROWS + threadIdx.x / G;
     const int64_t row = mine < g.rows ? mine : g.rows - 1;             // lanes without a row of their own repeat the last
-    const int lane = threadIdx.x % G, at = threadIdx.x & 63;
-    const uint64_t group = (G == 64 ? ~0ull : ((1ull << (G & 63)) - 1ull)) << (at - lane);
+    const int lane = threadIdx.x % G;
     const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
     R q;
 #pragma unroll
@@ -343,20 +403,20 @@ __global__ __launch_bounds__(256, 4) void k_sample_short(SampleArgs g) {
             broken |= !(q.x[k][e] < kInf);
             m = larger(q.x[k][e], m);
         }
-    m = group_max<G>(m);
-    broken = (__ballot(broken) & group) != 0 || s.c != s.c;
+    q.rank = lane;
+    q.shift = r.shift;
+    q.sh = &shared[threadIdx.x / G];
+    q.hist = q.sh->hist;
+    q.s = &s;
+    m = q.highest(m);
+    broken = q.some(broken) || s.c != s.c;
     const bool empty = m == -kInf;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int e = 0; e < N; ++e) q.w[k][e] = s.weight(q.x[k][e], empty ? 0.0f : m);
-    q.rank = lane;
-    q.shift = r.shift;
-    q.sh = &shared[threadIdx.x / G];
-    q.hist = q.sh->hist;
     q.good = !broken && !empty;
     q.m = m;
-    q.s = &s;
     if (q.any(!s.all())) {
         double total = 0.0;
         int allowed = 0;
@@ -370,8 +430,8 @@ __global__ __launch_bounds__(256, 4) void k_sample_short(SampleArgs g) {
                 allowed += is;
                 q.bottom = smaller(is ? q.x[k][e] : m, q.bottom);
             }
-        total = group_sum<G>(total);
-        allowed = group_sum<G>(allowed);
+        total = q.sum(total);
+        allowed = q.sum(allowed);
         q.bottom = q.lowest(q.bottom);
         if (q.any(s.k > 0 || s.p < 1.0)) {
             const Border b = border_of(q, s, m, total, allowed);
@@ -394,7 +454,7 @@ __global__ __launch_bounds__(256, 4) void k_sample_short(SampleArgs g) {
         part[k] = 0.0;
 #pragma unroll
         for (int e = 0; e < N; ++e) part[k] += q.w[k][e];
-        sums[k] = group_sum<G>(part[k]);
+        sums[k] = q.sum(part[k]);
         mass += sums[k];
     }
     const double aim = s.u * mass;
@@ -415,11 +475,12 @@ __global__ __launch_bounds__(256, 4) void k_sample_short(SampleArgs g) {
 #pragma unroll
             for (int e = 0; e < N; ++e) v[e] = q.w[k][e];
         }
-    const double upto = before + group_scan<G>(own);
-    const uint64_t over = __ballot(own > 0.0 && upto > aim) & group, some = __ballot(own > 0.0) & group;
+    const double upto = before + q.scan(own);
     // rounding may leave the aim at the end of the last mass: its lane, and its last entry, then
-    const int winner = over ? __ffsll((unsigned long long)over) - 1 : some ? 63 - __clzll((long long)some) : at - lane;
-    if (at != winner || mine >= g.rows) return;
+    int winner = q.first_of(own > 0.0 && upto > aim);
+    const int end = q.last_of(own > 0.0);
+    if (winner < 0) winner = end < 0 ? 0 : end;
+    if (lane != winner || mine >= g.rows) return;
     double sum = upto - own, found_w = 1.0;
     int found = -1;
     bool open = true;
@@ -989,10 +1050,16 @@ void launch_sample(const SampleArgs& g, hipStream_t s) {
     constexpr int K = 16 / Chunk<T>::N;                // 16 entries a lane
 #define SHORT(G)                                                                                                                \
     if (chunks <= G * K) {                                                                                                      \
-        hipLaunchKernelGGL((k_sample_short<T, MASK, G, K>), dim3((unsigned)((g.rows + 256 / G - 1) / (256 / G))), dim3(256), 0, s, g); \
+        constexpr int ROWS = G > 64 ? 1 : 256 / G;                                                                              \
+        hipLaunchKernelGGL((k_sample_short<T, MASK, G, K>), dim3((unsigned)((g.rows + ROWS - 1) / ROWS)), dim3(G > 64 ? G : 256), 0, s, g); \
         return;                                                                                                                 \
     }
     SHORT(4) SHORT(8) SHORT(16) SHORT(32) SHORT(64)
+    // From here to 4096 entries a row fits the registers of a block just as well; only a small top_k is quicker by the list of
+    // candidates (float32, 2^26 entries in rows of 1028 / 2048 / 4096: top_p 452 / 250 / 331 us against 1130 / 590 / 433 by list and
+    // whole row, top_k 40 402 / 214 / 241 against 273 / 144 / 90).
+    const bool few = !g.top_k && g.top_k_s > 0 && g.top_k_s <= 64;
+    if (!few) { SHORT(128) SHORT(256) }
 #undef SHORT
     const dim3 grid((unsigned)g.rows);
     const bool all = !g.temperature && !g.top_k && !g.top_p && !g.min_p && g.temperature_s >= 1.17549435e-38f && g.top_k_s <= 0 && g.top_p_s >= 1.0f && !(g.min_p_s > 0.0f);
@@ -1003,6 +1070,9 @@ void launch_sample(const SampleArgs& g, hipStream_t s) {
         hipLaunchKernelGGL((k_sample_list<T, MASK, THREADS, H>), grid, dim3(THREADS), 0, s, g);                                 \
         hipLaunchKernelGGL((k_sample_whole<T, MASK, THREADS, 0, true>), grid, dim3(THREADS), 0, s, g);                          \
     }
+    // Four blocks of 256 threads on a CU work on four rows in turn, one of 1024 on one: with many rows the former hide each other's
+    // waits (bfloat16 rows of 32000, top_p: 1024 of them 169 us against 216), with fewer than two a CU the latter is done sooner (256
+    // of them 59 us against 83).
     if (chunks <= 256 * 4) { LONG(256, 4) }
     else if (chunks <= 256 * 16 && g.rows >= 512) { LONG(256, 16) }
     else if (chunks <= 1024 * 4) { LONG(1024, 4) }

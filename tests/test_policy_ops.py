@@ -159,7 +159,7 @@ SETTINGS = [dict(), dict(temperature=0.6), dict(top_k=1), dict(top_k=5, temperat
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("vocab", [1, 2, 3, 19, 63, 64, 65, 255, 256, 257, 1000, 1025, 4099])
+@pytest.mark.parametrize("vocab", [1, 2, 3, 19, 63, 64, 65, 255, 256, 257, 1000, 1025, 1500, 2500, 4000, 4099])
 def test_draw(device, dtype, vocab):
     g = rng_of("draw", dtype, vocab)
     for n, s in enumerate(SETTINGS):
@@ -182,7 +182,7 @@ def test_draw_long_rows(device, dtype, vocab):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("vocab", [5, 64, 300, 5000, 40000])
+@pytest.mark.parametrize("vocab", [5, 64, 300, 1800, 3900, 5000, 40000])
 def test_draw_equal_logits(device, vocab):
     """Few different values: the border of every setting falls among equal entries, which go by lowest index."""
     g = rng_of("ties", vocab)
@@ -196,7 +196,7 @@ def test_draw_equal_logits(device, vocab):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("vocab", [4, 77, 700, 6000])
+@pytest.mark.parametrize("vocab", [4, 77, 700, 1500, 3500, 6000])
 def test_draw_masks_and_special_values(device, dtype, vocab):
     """Rows that a mask or -inf leaves empty, single entries, lowest and largest finite values, NaN and infinities behind the
     mask and in front of it."""
@@ -247,7 +247,7 @@ def test_draw_uniform_edges(device):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("vocab", [33, 900, 9000])
+@pytest.mark.parametrize("vocab", [33, 900, 1700, 3600, 9000])
 def test_draw_per_row_settings(device, vocab):
     g = rng_of("rows", vocab)
     lead = (3, 4)
@@ -388,7 +388,7 @@ def run_evaluation(x, a, gl, ge, **kw):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("vocab", [1, 2, 7, 19, 33, 64, 65, 128, 255, 513, 1024, 2050, 5003, 33001, 131075])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 19, 33, 64, 65, 128, 255, 513, 1024, 1500, 2050, 3001, 5003, 33001, 131075])
 def test_evaluation(device, dtype, vocab):
     g = rng_of("evaluate", dtype, vocab)
     for n, t in enumerate((1.0, 0.6, 2.5)):
@@ -401,7 +401,7 @@ def test_evaluation(device, dtype, vocab):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("vocab", [5, 60, 700, 9001])
+@pytest.mark.parametrize("vocab", [5, 60, 700, 1600, 9001])
 def test_evaluation_masks_and_special_values(device, dtype, vocab):
     g = rng_of("evaluate mask", dtype, vocab)
     rows = 16

@@ -3,9 +3,9 @@
 //
 // With the allowed entries A = {i : mask_i and x_i > -inf}, m = max_A x and w_i = exp((x_i - m) / T):
 //   draw      order A by (x falling, i rising); keep the first k, of these the shortest prefix that holds a share p of
-//             their mass, of these the entries with w_i >= min_p.  What is kept is a prefix of the order, so it is the set
-//             {x > tau} plus the first r entries equal to tau.  With W = its mass, the answer is the first i (by index)
-//             whose running mass exceeds u W; its log-probability is ln(w_i / W).
+//             their mass, of these the entries with w_i >= min_p.  What is kept is a prefix of the order: everything up to
+//             and with one entry.  With W = its mass, the answer is the first i (by index) whose running mass exceeds u W;
+//             its log-probability is ln(w_i / W).
 //   evaluate  s = sum_A w, t = sum_A w ln w: log p_a = ln w_a - ln s, H = ln s - t / s.
 //   gradient  d/dx_i = (gl (d_ia - p_i) - ge p_i (ln p_i + H)) / T.
 #pragma once

@@ -125,6 +125,7 @@ MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double 
         int count;
         double more;
         bool sure = !active, few = false;
+        int went = 0;                                  // one way only: sums of another order may differ in their last bit
         for (;;) {
             more = 0.0;
             double in = 0.0;
@@ -143,12 +144,12 @@ MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double 
             more = c.sum(more);
             in = c.sum(in);
             count = c.listed();
-            int to = b;
-            if (above + more >= aim && b > 0) to = b - 1;
-            else if (above + more + in < aim && b < LAST) to = b + 1;
-            else sure = true;
+            int go = 0;
+            if (above + more >= aim && b > 0) go = -1;
+            else if (above + more + in < aim && b < LAST) go = 1;
+            if (go == 0 || go == -went) sure = true;
             if (!c.any(active && !sure)) break;
-            b = sure ? b : to;
+            if (!sure) b += went = go;
         }
         few = count <= C::capacity;
         if (c.any(active && few)) {
@@ -214,6 +215,11 @@ MDP_DEV void wave_sync() {
 
 // Rows of up to G K chunks, 16 entries a lane: G lanes of a wave, or a block of G = 128 or 256, hold a row and its weights in
 // registers.  Groups of a wave go through their loops together until the last is done.
+//
+// Bound by instructions: 49152 x 256 float32 with top_p takes 44 us, 1730 vector instructions for a wave's four rows (300 of them the
+// weights), where the 50 MB are 11 us at the copy rate; uncut it takes 20.  Searching the border by halving the value range, sixteen
+// compares and 64-bit adds a step, took 71.  The registers that hold entries and weights leave four waves a SIMD; with five (96
+// registers) what spills costs more: 53.
 template <typename T, int G, int K>
 struct ShortRow {
     static constexpr int N = Chunk<T>::N, size = G, capacity = G;
@@ -347,19 +353,18 @@ struct ShortRow {
     template <bool COUNT>
     MDP_DEV Border last_kept(int n, double above, double aim) const {
         const bool in = rank < n;
-        const uint64_t mine = in ? sh->list[rank].word : ~0ull;
-        double before = above;
+        const Listed mine = in ? sh->list[rank] : Listed{~0ull, 0.0};
         int order = 0;
-        for (int j = 0; G <= 64 ? __any(j < n) != 0 : j < n; ++j) {
-            const Listed o = sh->list[j];              // beyond n: what was there before
-            const bool first = j < n && o.word < mine;
-            before += first ? o.value : 0.0;
-            order += first;
-        }
+        for (int j = 0; G <= 64 ? __any(j < n) != 0 : j < n; ++j) order += j < n && sh->list[j].word < mine.word;
+        sync();
+        if (in) sh->list[order] = mine;                // in order now, however they came
+        sync();
+        const Listed at = in ? sh->list[rank] : Listed{~0ull, 0.0};
+        const double before = above + (scan(at.value) - at.value);
         int kept = sum((int)(in && before < aim));
         kept = kept ? kept : 1;
-        const bool me = in && order == kept - 1;
-        return Border{highest(me ? value_of(mine) : -kInf), sum(me ? (int)(uint32_t)mine : 0)};
+        const bool me = in && rank == kept - 1;
+        return Border{highest(me ? value_of(at.word) : -kInf), sum(me ? (int)(uint32_t)at.word : 0)};
     }
     MDP_DEV int nth_equal(float v, int r) const {
         int seen = 0, at = 0;
@@ -505,6 +510,11 @@ __global__ __launch_bounds__(G > 64 ? G : 256, 4) void k_sample_short(SampleArgs
 // already hold a share p of the row's mass, is not above the border.  The entries from there on -- a few more than are kept -- are
 // gathered in index order, sorted, and everything exact happens on them.  Where no such value exists or too many entries lie above
 // it (flat rows), the border is searched over the whole row.
+//
+// 1024 x 131072 bfloat16 with top_p and min_p: 142 us for 268 MB (57 at the copy rate).  A row fills the registers of a CU, so while
+// it arrives (13 us of its share of the memory rate) nothing is left to do but its maxima and 32-bit mass, and the 15 us after it --
+// bound, list, sort -- load nothing.  Uncut rows of that size: 160 us, 64-bit weights of every entry; rows that the list leaves:
+// 690 us (scale 0.5), five passes, of which all but the first read the row again from the caches.
 template <typename T, bool MASK, int THREADS, int H>
 struct LongRow {
     static constexpr int N = Chunk<T>::N, W = THREADS / 64, size = THREADS, capacity = THREADS;

@@ -265,6 +265,20 @@ def test_draw_per_row_settings(device, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows, vocab, scale", [(3000, 40, 0.1), (700, 1000, 0.3), (300, 3000, 2.0), (100, 9000, 0.2), (40, 70001, 1.0)])
+def test_draw_repeats_itself(device, rows, vocab, scale):
+    """The same call gives the same bits, whatever order its lanes list entries in."""
+    g = rng_of("again", vocab)
+    x = (torch.randn(rows, vocab, generator=g) * scale).to(torch.bfloat16).to(device)
+    u = torch.rand(rows, generator=g).to(device)
+    first = rl.sample_categorical(x, u, top_p=0.7, top_k=vocab // 2)
+    check_draw(x[:4], u[:4], (first[0][:4], first[1][:4]), top_p=0.7, top_k=vocab // 2)
+    for _ in range(4):
+        again = rl.sample_categorical(x, u, top_p=0.7, top_k=vocab // 2)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.gpu
 def test_draw_layouts(device):
     """Any strides and offsets, one row, no rows, an expanded row, a non-default stream."""
     g = rng_of("layout")

@@ -88,7 +88,8 @@ def sample_categorical(logits: torch.Tensor, u: torch.Tensor | None = None, *, t
 
     ``u`` (float32, leading shape, in [0, 1)) makes the draw: the answer is the first kept entry, by index, up to which the
     kept entries hold more than a share ``u`` of their weight ``exp(logit / temperature)``.  Without it the numbers come from
-    the device generator of ``isaaclab_amd.utils.math`` (``seed_samplers``), fresh on every replay of a captured call.
+    the device generator of ``isaaclab_amd.utils.math`` (``seed_samplers``; seeded, or drawn from, before a capture), fresh on
+    every replay of a captured call.
 
     Kept are the ``top_k`` largest allowed logits (0: all; equal ones by lowest index), of these the fewest largest that hold a
     share ``top_p`` of their weight (one at least), of these the ones of at least ``min_p`` times the largest weight.
@@ -103,6 +104,8 @@ def sample_categorical(logits: torch.Tensor, u: torch.Tensor | None = None, *, t
     lead = logits.shape[:-1]
     t_t, t_s = _setting(temperature, "temperature", torch.float32, logits, 0.0, _MOST)
     k_t, k_s = _setting(top_k, "top_k", torch.int32, logits, 0, 2147483647)
+    if k_s != int(k_s):
+        raise ValueError(f"top_k must be a whole number, got {k_s}")
     p_t, p_s = _setting(top_p, "top_p", torch.float32, logits, 0.0, 1.0)
     q_t, q_s = _setting(min_p, "min_p", torch.float32, logits, 0.0, 1.0)
     state = None

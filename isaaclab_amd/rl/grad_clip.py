@@ -9,6 +9,8 @@ import torch
 from .. import _lib as L
 
 _DTYPES = L.DTYPES
+_contiguous, _device = torch.Tensor.is_contiguous, torch.Tensor.get_device
+_address, _count = torch.Tensor.data_ptr, torch.Tensor.numel
 _KINDS = {2.0: 2, 1.0: 1, float("inf"): 0}
 
 
@@ -51,23 +53,25 @@ def _table(grads: list, outs: list | None) -> tuple[array, int]:
     try:
         index = grads[0].get_device()
         kinds = [_DTYPES[t.dtype] for t in grads]
-        plain = all([t.is_contiguous() for t in grads])
+        plain = index >= 0 and all(map(_contiguous, grads)) and set(map(_device, grads)) == {index}
         if outs is None:
             outs, to = grads, kinds
         else:
             to = [_DTYPES[t.dtype] for t in outs]
-            plain = (plain and all([t.is_contiguous() for t in outs]) and [t.shape for t in outs] == [t.shape for t in grads]
-                     and all([o == k or o == 0 for o, k in zip(to, kinds)]) and {t.get_device() for t in outs} == {index})
-        plain = plain and index >= 0 and {t.get_device() for t in grads} == {index}
-    except (AttributeError, KeyError, RuntimeError):
+            plain = (plain and all(map(_contiguous, outs)) and [t.shape for t in outs] == [t.shape for t in grads]
+                     and all([o == k or o == 0 for o, k in zip(to, kinds)]) and set(map(_device, outs)) == {index})
+    except (AttributeError, KeyError, RuntimeError, TypeError):
         plain = False
     if not plain:                            # something to refuse, or strides that take a closer look
         _check_all(grads, outs or grads)
-        index = grads[0].get_device()
-        kinds, to = [_DTYPES[t.dtype] for t in grads], [_DTYPES[t.dtype] for t in outs or grads]
-        outs = outs or grads
-    words = [w for g, o, k, u in zip(grads, outs, kinds, to) for w in (g.data_ptr(), o.data_ptr(), g.numel(), k | u << 32)]
-    return array("q", words), index
+        index, outs = grads[0].get_device(), outs or grads
+        kinds, to = [_DTYPES[t.dtype] for t in grads], [_DTYPES[t.dtype] for t in outs]
+    table = array("q", bytes(32 * len(grads)))
+    table[0::4] = array("q", map(_address, grads))
+    table[1::4] = table[0::4] if outs is grads else array("q", map(_address, outs))
+    table[2::4] = array("q", map(_count, grads))
+    table[3::4] = array("q", [k | o << 32 for k, o in zip(kinds, to)])
+    return table, index
 
 
 def _check_all(grads: list, outs: list):

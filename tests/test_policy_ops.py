@@ -57,8 +57,8 @@ def test_oracle_against_torch():
     (grad,) = torch.autograd.grad((lp, h), x, (gl, ge))
     for r in range(6):
         got = O.evaluate_row(x[r].detach().numpy(), int(a[r]), None, 0.7, float(gl[r]), float(ge[r]))
-        np.testing.assert_allclose(got[0], float(lp[r]), rtol=1e-12)
-        np.testing.assert_allclose(got[1], float(h[r]), rtol=1e-12)
+        np.testing.assert_allclose(got[0], lp[r].item(), rtol=1e-12)
+        np.testing.assert_allclose(got[1], h[r].item(), rtol=1e-12)
         np.testing.assert_allclose(got[2], grad[r].numpy(), rtol=1e-10, atol=1e-14)
     # kept entries by hand: weights 4, 2, 1, 1 of 8
     x = np.log(np.array([1.0, 4.0, 1.0, 2.0]))
@@ -341,6 +341,7 @@ def test_draw_refusals(device):
                         ("temperature", lambda: rl.sample_categorical(x, u, temperature=-0.5)),
                         ("temperature", lambda: rl.sample_categorical(x, u, temperature=math.nan)),
                         ("top_k", lambda: rl.sample_categorical(x, u, top_k=-1)),
+                        ("whole number", lambda: rl.sample_categorical(x, u, top_k=2.5)),
                         ("top_p", lambda: rl.sample_categorical(x, u, top_p=1.5)),
                         ("min_p", lambda: rl.sample_categorical(x, u, min_p=-0.1)),
                         ("top_p of shape", lambda: rl.sample_categorical(x, u, top_p=torch.ones(3, device=device))),

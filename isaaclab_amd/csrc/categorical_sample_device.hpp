@@ -56,14 +56,14 @@ MDP_DEV void anew(V& x) { asm volatile("" : "+v"(x)); }
 //   each(f): f(x, place, w) for each of this lane's entries, w() its weight; sort_in(bucket, f): f(bucket of x, w) for each, and
 //   each_sorted(bucket, f): f(x, place, w, bucket of x) after it; weight(x); sum, highest, lowest over all; scan: the sum over the
 //   lanes up to and with this one; sync; any: over the lanes that run this loop in step; size, rank: lanes and this lane's number;
-//   hist[per_lane size] in shared memory, and there a list of up to `capacity` entries: put<COUNT>(x, place, w) adds one, listed() tells how
-//   many were put, last_kept<COUNT>(n, above, aim) finds the border among the n listed, with `above` before them; nth_equal(x, r):
-//   the place of the r-th entry equal to x (r from 1).
+//   hist[per_lane size] in shared memory, and there a list of up to `capacity` entries: put<COUNT>(x, place, w) adds one, listed()
+//   tells how many were put, last_kept<COUNT>(n, above, aim) finds the border among the n listed, with `above` before them;
+//   nth_equal(x, r): the place of the r-th entry equal to x (r from 1); bottom: the row's lowest entry.
 // Entries are sorted into buckets that fall with the value: about the maximum first, a bucket a small part of a binary order of
-// magnitude or of what the row spans (entries more than `window` orders below share the last); bottom: the row's lowest entry.  The bucket in which the aim is reached, by 32-bit fixed point, is confirmed
-// in 64 bits while its few entries are listed, and these are looked at one by one.  If they are too many, the bucket is cut again,
-// by keys, which ends with one value.  Where `total`, the mass of the row, is known in 32 bits only (C::total_known false) and the aim
-// is a share of it (share_of_total), the first pass sums it up in 64.
+// magnitude or of what the row spans (entries more than `window` orders below share the last).  The bucket in which the aim is
+// reached, by 32-bit fixed point, is confirmed in 64 bits while its few entries are listed, and these are looked at one by one.  If
+// they are too many, the bucket is cut again, by keys, which ends with one value.  Where `total`, the mass of the row, is known in 32
+// bits only (C::total_known false) and the aim is a share of it (share_of_total), the first pass sums it up in 64.
 template <bool COUNT, class C>
 MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double total, bool share_of_total, bool active) {
     constexpr int PER = C::per_lane, LAST = PER * C::size - 2, NONE = PER * C::size - 1;   // the last bucket; an entry that is in none
@@ -508,8 +508,8 @@ __global__ __launch_bounds__(G > 64 ? G : 256, 4) void k_sample_short(SampleArgs
 // A question over a long row is dear (131072 bfloat16 entries: 9 us of a CU in 32 bits), so what k, p and min_p keep is looked for
 // among few candidates: the threads' own largest entries are a part of the row, so a value above which THEY already are k, or
 // already hold a share p of the row's mass, is not above the border.  The entries from there on -- a few more than are kept -- are
-// gathered in index order, sorted, and everything exact happens on them.  Where no such value exists or too many entries lie above
-// it (flat rows), the border is searched over the whole row.
+// listed and sorted, and everything exact happens on them.  Where no such value exists or too many entries lie above it (flat rows),
+// the border is searched over the whole row.
 //
 // 1024 x 131072 bfloat16 with top_p and min_p: 142 us for 268 MB (57 at the copy rate).  A row fills the registers of a CU, so while
 // it arrives (13 us of its share of the memory rate) nothing is left to do but its maxima and 32-bit mass, and the 15 us after it --
@@ -521,7 +521,10 @@ struct LongRow {
     static constexpr int per_lane = 4;
     static constexpr float window = 24.0f;
     static constexpr bool total_known = false;
-    static constexpr double kLess = 1.0 - 1.53e-5, kMore = 1.0 + 1.53e-5;    // 2^-16: what the mass in 32 bits may be off
+    // What the mass in 32 bits may be off, as a share: 2^-16 for the weights (three roundings of an exponent of 20 binary orders, the
+    // orders that hold the mass of 2^18 entries, make 2.4e-6, sums of chunks as much again), and two roundings for each time that a
+    // thread's largest entry changed.
+    MDP_DEV double rough() const { return 1.53e-5 + 2.4e-7 * (double)steps; }
     struct Shared {
         double d[W + 1];
         int n[W + 1];
@@ -672,7 +675,7 @@ struct LongRow {
                 v[i] = sh.maxima.top[i * 64 + lane];
                 w[i] = __builtin_amdgcn_exp2f(larger((v[i] - m) * c, -300.0f));
             }
-            const float aim = (float)s.p * mass * 1.0001f;             // above p S whatever 32 bits made of the sums
+            const float aim = (float)s.p * mass * (1.0001f + 1e-6f * (float)steps);    // above p S whatever 32 bits made of the sums
             float bound = -kInf;
             if (s.k > 0 || s.p < 1.0) {
                 const auto enough = [&](float from) {
@@ -794,11 +797,12 @@ struct LongRow {
     }
     MDP_DEV static int votes(bool v) { return __popcll(__ballot(v)); }
     // how many of a wave's sorted entries are kept, by what `held` weighs; -1 if that is only the 32-bit mass and too near to tell
-    MDP_DEV int kept_of_few(int n, double ws, double before, double held, bool rough) const {
+    MDP_DEV int kept_of_few(int n, double ws, double before, double held, bool in_32) const {
+        const double off = rough();
         int kept = s.k > 0 ? min(s.k, n) : n;
         if (s.p < 1.0) {
             const int short_of = votes(lane < kept && before < s.p * held);
-            if (rough && (votes(lane < kept && before < s.p * held * kLess) != short_of || votes(lane < kept && before < s.p * held * kMore) != short_of)) return -1;
+            if (in_32 && (votes(lane < kept && before < s.p * held * (1.0 - off)) != short_of || votes(lane < kept && before < s.p * held * (1.0 + off)) != short_of)) return -1;
             kept = min(kept, short_of);
         }
         return max(1, min(kept, votes(lane < n && ws >= s.mp)));
@@ -854,8 +858,9 @@ struct LongRow {
             int short_of = block_sum((int)(tid < kept && before < s.p * held));
             if (s.k == 0) {
                 // the row's mass in 32 bits decides unless the border is within its error of the aim
-                const int low = block_sum((int)(tid < kept && before < s.p * held * kLess));
-                const int high = block_sum((int)(tid < kept && before < s.p * held * kMore));
+                const double off = rough();
+                const int low = block_sum((int)(tid < kept && before < s.p * held * (1.0 - off)));
+                const int high = block_sum((int)(tid < kept && before < s.p * held * (1.0 + off)));
                 if (low != high) {
                     held = exact_mass();
                     short_of = block_sum((int)(tid < kept && before < s.p * held));

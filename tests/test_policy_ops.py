@@ -265,6 +265,19 @@ def test_draw_per_row_settings(device, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [700, 3000, 9001, 70001, 300007])
+def test_draw_rising_and_falling_rows(device, vocab):
+    """Rows in order of their values: the largest entry so far changes with every entry, or never; the border is a place."""
+    line = torch.linspace(-7.0, 7.0, vocab)
+    step = torch.arange(vocab) * 1e-7
+    x = torch.stack([line, line.flip(0), step, step.flip(0), (line * 1e-3), line ** 3 / 10]).to(device)
+    for s in (dict(top_p=0.5), dict(top_p=0.93, temperature=0.3), dict(top_k=vocab // 3, top_p=0.8), dict(min_p=0.3), dict()):
+        for shift in (0.0, 0.61):
+            u = torch.tensor([0.1, 0.25, 0.4, 0.5, 0.7, 0.9], device=device).add(shift).remainder(1.0)
+            check_draw(x, u, rl.sample_categorical(x, u, **s), **s)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows, vocab, scale", [(3000, 40, 0.1), (700, 1000, 0.3), (300, 3000, 2.0), (100, 9000, 0.2), (40, 70001, 1.0)])
 def test_draw_repeats_itself(device, rows, vocab, scale):
     """The same call gives the same bits, whatever order its lanes list entries in."""

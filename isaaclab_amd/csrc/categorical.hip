@@ -377,7 +377,7 @@ extern "C" int mdp_categorical_sample(const mdp_categorical_sample_t* a, void* s
         by_rows(a->rows, [&](int64_t at, int64_t rows) {
             const SampleArgs g{(const T*)a->logits + at * a->ld, a->ld, offset(a->mask, at * a->ld_mask), a->ld_mask, (int)a->vocab,
                                rows, at, offset(a->temperature, at), offset(a->top_k, at), offset(a->top_p, at), offset(a->min_p, at),
-                               a->temperature_scalar, a->top_k_scalar, a->top_p_scalar, a->min_p_scalar, offset(a->u, at),
+                               rate_of(a->temperature_scalar), a->top_k_scalar, a->top_p_scalar, a->min_p_scalar, offset(a->u, at),
                                (const unsigned long long*)a->state, a->actions + at, a->log_prob + at};
             launch_sample<T, decltype(m)::value>(g, s);
         });

@@ -194,13 +194,24 @@ int most_chunks(const void* logits, int64_t ld, int64_t rows, int vocab) {
     return (vocab + (aligned ? 0 : N - 1) + N - 1) / N;
 }
 
+// log2(e) / T in 64 bits: a NaN for a temperature that is negative or NaN, kGreedy for one below the smallest normal number, never
+// 0, so that -inf times it stays -inf.  A 64-bit division takes some forty instructions: for one temperature the host makes it.
+constexpr double kGreedy = 1e300;
+__host__ __device__ inline double rate_of(float t) {
+    if (!(t >= 0.0f)) return __builtin_nan("");
+    if (t < 1.17549435e-38f) return kGreedy;
+    const double c = 1.4426950408889634 / (double)t;
+    return c > 1e-300 ? c : 1e-300;
+}
+
 struct SampleArgs {
     const void* logits; int64_t ld;
     const uint8_t* mask; int64_t ld_mask;
     int vocab; int64_t rows;
     int64_t row0;                                      // of the call's rows the launch's first
     const float* temperature; const int* top_k; const float* top_p; const float* min_p;
-    float temperature_s; int top_k_s; float top_p_s; float min_p_s;
+    double rate;                                       // rate_of() the temperature that all rows share
+    int top_k_s; float top_p_s; float min_p_s;
     const float* u; const unsigned long long* state;
     int64_t* actions; float* log_prob;
 };

@@ -17,16 +17,13 @@ struct Settings {
     double p, mp;                                      // p = 1, mp = 0: no limit
     double u;
     MDP_DEV Settings(const SampleArgs& g, int64_t row) {
-        const float t = g.temperature ? g.temperature[row] : g.temperature_s;
         k = g.top_k ? g.top_k[row] : g.top_k_s;
         float pf = g.top_p ? g.top_p[row] : g.top_p_s, mf = g.min_p ? g.min_p[row] : g.min_p_s;
         if (k < 0) k = 0;
         p = pf < 1.0f ? (pf > 0.0f ? (double)pf : 0.0) : 1.0;
         mp = mf > 0.0f ? (mf < 1.0f ? (double)mf : 1.0) : 0.0;
-        c = 1.4426950408889634 / (double)t;
-        c = c > 1e-300 ? c : 1e-300;                   // infinite temperature: -inf * c stays -inf
-        if (t >= 0.0f && t < 1.17549435e-38f) { c = 1e300; k = 1; p = 1.0; mp = 0.0; }
-        if (!(t >= 0.0f)) c = __builtin_nan("");
+        c = g.temperature ? rate_of(g.temperature[row]) : g.rate;
+        if (c == kGreedy) { k = 1; p = 1.0; mp = 0.0; }
         float uf = g.u ? g.u[row] : u01(rng4(g.state[0], g.state[1], kStream, (uint64_t)(g.row0 + row)).x);
         u = uf > 0.0f ? (uf < 0.99999994f ? (double)uf : 0.99999994039535522) : 0.0;
     }
@@ -423,22 +420,26 @@ __global__ __launch_bounds__(G > 64 ? G : 256, 4) void k_sample_short(SampleArgs
     q.good = !broken && !empty;
     q.m = m;
     if (q.any(!s.all())) {
-        double total = 0.0;
-        int allowed = 0;
-        q.bottom = m;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                total += q.w[k][e];
-                const bool is = q.x[k][e] > -kInf;
-                allowed += is;
-                q.bottom = smaller(is ? q.x[k][e] : m, q.bottom);
-            }
-        total = q.sum(total);
-        allowed = q.sum(allowed);
-        q.bottom = q.lowest(q.bottom);
         if (q.any(s.k > 0 || s.p < 1.0)) {
+            double total = 0.0;
+            int allowed = 0;
+            q.bottom = m;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    total += q.w[k][e];
+                    q.bottom = smaller(q.x[k][e] > -kInf ? q.x[k][e] : m, q.bottom);
+                }
+            total = q.sum(total);
+            q.bottom = q.lowest(q.bottom);
+            if (q.any(s.k > 0)) {
+#pragma unroll
+                for (int k = 0; k < K; ++k)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) allowed += q.x[k][e] > -kInf;
+                allowed = q.sum(allowed);
+            }
             const Border b = border_of(q, s, m, total, allowed);
 #pragma unroll
             for (int k = 0; k < K; ++k)
@@ -1077,7 +1078,7 @@ void launch_sample(const SampleArgs& g, hipStream_t s) {
     if (!few) { SHORT(128) SHORT(256) }
 #undef SHORT
     const dim3 grid((unsigned)g.rows);
-    const bool all = !g.temperature && !g.top_k && !g.top_p && !g.min_p && g.temperature_s >= 1.17549435e-38f && g.top_k_s <= 0 && g.top_p_s >= 1.0f && !(g.min_p_s > 0.0f);
+    const bool all = !g.temperature && !g.top_k && !g.top_p && !g.min_p && g.rate != kGreedy && g.rate == g.rate && g.top_k_s <= 0 && g.top_p_s >= 1.0f && !(g.min_p_s > 0.0f);
 #define LONG(THREADS, H)                                                                                                        \
     if (all) {                                                                                                                  \
         hipLaunchKernelGGL((k_sample_whole<T, MASK, THREADS, H, false>), grid, dim3(THREADS), 0, s, g);                         \

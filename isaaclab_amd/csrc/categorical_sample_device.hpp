@@ -32,14 +32,6 @@ struct Settings {
     MDP_DEV double weight(float x, float m) const { return exp2_neg(((double)x - (double)m) * c); }
 };
 
-// What is kept is a prefix of the row sorted by (value falling, place rising): everything up to and with one entry.
-struct Border {
-    float tau;
-    int place;
-    MDP_DEV bool keeps(float x, int i) const { return x > tau || (x == tau && i <= place); }
-};
-MDP_DEV Border everything() { return Border{-__FLT_MAX__, 0x7fffffff}; }
-
 // an entry as a word that rises in the order (value falling, place rising)
 MDP_DEV uint64_t word_of(float x, int place) { return (uint64_t)(~key_of(x)) << 32 | (uint32_t)place; }
 MDP_DEV float value_of(uint64_t word) { return of_key(~(uint32_t)(word >> 32)); }
@@ -48,160 +40,11 @@ MDP_DEV float value_of(uint64_t word) { return of_key(~(uint32_t)(word >> 32)); 
 template <typename V>
 MDP_DEV void anew(V& x) { asm volatile("" : "+v"(x)); }
 
-// Finds the last entry of the shortest prefix that holds `aim`, counting entries (COUNT) or their weights.  C is what searches a row
-// together -- a group of lanes or a block -- and gives
-//   each(f): f(x, place, w) for each of this lane's entries, w() its weight; sort_in(bucket, f): f(bucket of x, w) for each, and
-//   each_sorted(bucket, f): f(x, place, w, bucket of x) after it; weight(x); sum, highest, lowest over all; scan: the sum over the
-//   lanes up to and with this one; sync; any: over the lanes that run this loop in step; size, rank: lanes and this lane's number;
-//   hist[per_lane size] in shared memory, and there a list of up to `capacity` entries: put<COUNT>(x, place, w) adds one, listed()
-//   tells how many were put, last_kept<COUNT>(n, above, aim) finds the border among the n listed, with `above` before them;
-//   nth_equal(x, r): the place of the r-th entry equal to x (r from 1); bottom: the row's lowest entry.
-// Entries are sorted into buckets that fall with the value: about the maximum first, a bucket a small part of a binary order of
-// magnitude or of what the row spans (entries more than `window` orders below share the last).  The bucket in which the aim is
-// reached, by 32-bit fixed point, is confirmed in 64 bits while its few entries are listed, and these are looked at one by one.  If
-// they are too many, the bucket is cut again, by keys, which ends with one value.  Where `total`, the mass of the row, is known in 32
-// bits only (C::total_known false) and the aim is a share of it (share_of_total), the first pass sums it up in 64.
-template <bool COUNT, class C>
-MDP_DEV Border find_border(C& c, const Settings& s, float m, double aim, double total, bool share_of_total, bool active) {
-    constexpr int PER = C::per_lane, LAST = PER * C::size - 2, NONE = PER * C::size - 1;   // the last bucket; an entry that is in none
-    Border border = everything();
-    aim = fmax(aim, 1e-300);                           // the first entry reaches a share of 0
-    float per = (float)LAST / fmaxf(fminf(C::window / s.c32(), m - c.bottom), 1e-30f);   // buckets for a difference of 1
-    double scale = COUNT ? 1.0 : 2147483648.0 / total;                  // all weights together: half of what 32 bits hold
-    float top = m, bottom = -__FLT_MAX__;
-    double above = 0.0;
-    int shift = -1;                                    // by value; later by key >> shift
-    const auto by_value = [&](float x) { return x > -kInf ? (int)fminf((top - x) * per, (float)LAST) : NONE; };
-    const auto bucket = [&](float x) {
-        if (shift < 0) return by_value(x);
-        float again = x;
-        anew(again);
-        return x <= top && x >= bottom ? (int)((key_of(top) - key_of(again)) >> shift) : NONE;
-    };
-    while (c.any(active)) {
-        c.sync();
-        for (int i = 0; i < PER; ++i) c.hist[c.rank * PER + i] = 0u;
-        c.sync();
-        anew(per);
-        anew(scale);
-        double weighed = 0.0;
-        const auto count_in = [&](int b, auto&& w) {
-            const double v = COUNT ? 1.0 : w();
-            if (!COUNT && !C::total_known) weighed += v;
-            if (active && b != NONE) atomicAdd(&c.hist[b], COUNT ? 1u : (uint32_t)fma(v, scale, 0.5));
-        };
-        if (c.any(active && shift >= 0)) c.sort_in(bucket, count_in);
-        else c.sort_in(by_value, count_in);
-        c.sync();
-        if (!COUNT && !C::total_known && share_of_total) {
-            aim = fmax(s.p * c.sum(weighed), 1e-300);
-            share_of_total = false;
-        }
-        const double need_d = fmin(fmax((aim - above) * scale, 1.0), 4294967295.0);
-        const uint32_t need = (uint32_t)__builtin_ceil(need_d);
-        uint32_t q[PER], mine = 0u;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            q[i] = c.hist[c.rank * PER + i];
-            mine += q[i];
-        }
-        uint32_t run = c.scan(mine) - mine;
-        int b = NONE, full = -1;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            run += q[i];
-            if (b == NONE && run >= need) b = c.rank * PER + i;
-            if (q[i]) full = c.rank * PER + i;
-        }
-        b = (int)c.lowest((float)b);
-        if (c.any(active && b == NONE)) {              // the aim in the rounding of the last ones: the last that holds anything
-            full = (int)c.highest((float)full);
-            if (b == NONE) b = full < 0 ? LAST : full;
-        }
-        // confirm: the bucket is not the one while the entries above it reach the aim by themselves, or fall short of it with its own
-        int count;
-        double more;
-        bool sure = !active, few = false;
-        int went = 0;                                  // one way only: sums of another order may differ in their last bit
-        for (;;) {
-            more = 0.0;
-            double in = 0.0;
-            c.sync();
-            c.clear_list();
-            c.sync();
-            c.each_sorted(bucket, [&](float x, int i, auto&& w, int at) {
-                const double v = COUNT ? 1.0 : w();
-                more += at < b ? v : 0.0;
-                if (at == b) {
-                    in += v;
-                    if (active) c.template put<COUNT>(x, i, v);
-                }
-            });
-            c.sync();
-            more = c.sum(more);
-            in = c.sum(in);
-            count = c.listed();
-            int go = 0;
-            if (above + more >= aim && b > 0) go = -1;
-            else if (above + more + in < aim && b < LAST) go = 1;
-            if (go == 0 || go == -went) sure = true;
-            if (!c.any(active && !sure)) break;
-            if (!sure) b += went = go;
-        }
-        few = count <= C::capacity;
-        if (c.any(active && few)) {
-            const Border found = c.template last_kept<COUNT>(active && few ? count : 0, above + more, aim);
-            if (active && few) border = found;
-        }
-        if (c.any(active && !few)) {
-            float hi = -kInf, lo = kInf;
-            c.each_sorted(bucket, [&](float x, int, auto&&, int at) {
-                if (at == b) { hi = fmaxf(hi, x); lo = fminf(lo, x); }
-            });
-            hi = c.highest(hi);
-            lo = c.lowest(lo);
-            const bool one = hi == lo;
-            if (c.any(active && !few && one)) {
-                const double v = COUNT ? 1.0 : c.weight(hi), want = (aim - (above + more)) / v;
-                const int r = want < 1.0 ? 1 : want < (double)count ? (int)__builtin_ceil(want) : count;
-                const int place = c.nth_equal(hi, r);
-                if (active && !few && one) border = Border{hi, place};
-            }
-            if (!few && !one) {
-                top = hi;
-                bottom = lo;
-                above += more;
-                const uint32_t range = key_of(hi) - key_of(lo);
-                shift = 0;
-                while (range >> shift > (uint32_t)LAST) ++shift;
-            }
-            active = active && !few && !one;
-        } else active = false;
-    }
-    return border;
-}
+}  // namespace mdp
 
-// The border that k and p draw together, of `allowed` entries that weigh `total`.
-template <class C>
-MDP_DEV Border border_of(C& c, const Settings& s, float m, double total, int allowed) {
-    Border b = everything();
-    const bool by_k = s.k > 0 && s.k < allowed, by_p = s.p < 1.0;
-    double held = total;
-    if (c.any(by_k)) {
-        const Border f = find_border<true>(c, s, m, (double)s.k, 1.0, false, by_k);
-        if (by_k) b = f;
-        if (c.any(by_k && by_p)) {
-            double kept = 0.0;
-            c.each([&](float x, int i, auto&& w) { kept += b.keeps(x, i) ? w() : 0.0; });
-            held = c.sum(kept);
-        }
-    }
-    if (c.any(by_p)) {
-        const Border f = find_border<false>(c, s, m, s.p * held, total, !by_k, by_p);
-        if (by_p && (f.tau > b.tau || (f.tau == b.tau && f.place < b.place))) b = f;
-    }
-    return b;
-}
+#include "categorical_border_device.hpp"
+
+namespace mdp {
 
 // Shared memory that lanes of one wave pass to each other: no barrier, only the order of its accesses
 MDP_DEV void wave_sync() {
@@ -262,18 +105,24 @@ struct ShortRow {
             else f(i, __builtin_bit_cast(V, sh->u[i]));
         }
     }
+    // what is the same for all lanes of a wave, in scalar registers
+    template <typename V>
+    MDP_DEV static V shared_by_all(V v) {
+        if constexpr (G < 64) return v;
+        else return of_lane(v, 0);
+    }
     template <typename V>
     MDP_DEV V sum(V v) const {
-        if constexpr (G <= 64) return group_sum<G>(v);
+        if constexpr (G <= 64) return shared_by_all(group_sum<G>(v));
         V all = V(0);
         exchange(group_sum<64>(v), (threadIdx.x & 63) == 0, [&](int, V o) { all += o; });
-        return all;
+        return shared_by_all(all);
     }
     MDP_DEV float highest(float v) const {
-        if constexpr (G <= 64) return group_max<G>(v);
+        if constexpr (G <= 64) return shared_by_all(group_max<G>(v));
         float all = -kInf;
         exchange(group_max<64>(v), (threadIdx.x & 63) == 0, [&](int, float o) { all = larger(o, all); });
-        return all;
+        return shared_by_all(all);
     }
     MDP_DEV float lowest(float v) const { return -highest(-v); }
     template <typename V>
@@ -340,7 +189,7 @@ struct ShortRow {
         }
     }
     MDP_DEV void clear_list() const { if (rank == 0) sh->n = 0; }
-    MDP_DEV int listed() const { return sh->n; }
+    MDP_DEV int listed() const { return shared_by_all(sh->n); }
     template <bool COUNT>
     MDP_DEV void put(float v, int i, double value) const {
         anew(v);
@@ -388,7 +237,9 @@ __global__ __launch_bounds__(G > 64 ? G : 256, 4) void k_sample_short(SampleArgs
     using R = ShortRow<T, G, K>;
     constexpr int N = Chunk<T>::N, ROWS = G > 64 ? 1 : 256 / G;
     __shared__ typename R::Shared shared[ROWS];
-    const int64_t mine = (int64_t)blockIdx.x * ROWS + threadIdx.x / G;
+    // of a row that takes whole waves, what its lanes share stands in scalar registers
+    const int in_block = threadIdx.x / G;
+    const int64_t mine = (int64_t)blockIdx.x * ROWS + (G < 64 ? in_block : __builtin_amdgcn_readfirstlane(in_block));
     const int64_t row = mine < g.rows ? mine : g.rows - 1;             // lanes without a row of their own repeat the last
     const int lane = threadIdx.x % G;
     const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);

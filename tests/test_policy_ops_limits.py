@@ -1,0 +1,29 @@
+"""The policy-side operators at the ends of their ranges: rows of -inf, the smallest temperatures and weights, peaks over long tails,
+the longest rows with masks and in large batches, tolerances derived from the kernels' own roundings.
+
+U = 2^-24 is half a step of float32; helpers and the float64 definitions are those of test_policy_ops.py."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import isaaclab_amd._lib as L
+from isaaclab_amd import rl
+from oracle import policy_np as O
+from test_policy_ops import DT, U, check_draw, check_evaluation, f64, f32v, rng_of, run_evaluation
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [60, 700, 3000, 9001, 131072])
+def test_draw_peaks_over_long_tails(device, vocab):
+    """The border lies in a tail whose entries weigh less than 2^-32 of the row: found by a few cuts (the host program of
+    test_border_search.py counts them)."""
+    g = rng_of("peak", vocab)
+    x = torch.randn(6, vocab, generator=g) * 0.1
+    for r, peak in enumerate((10.0, 15.0, 20.0, 22.8, 23.0, 30.0)):
+        x[r, vocab // 3 + r] = peak
+    x = x.to(device)
+    for p in (0.9999, 0.99995, 0.99999, 1 - 2.0 ** -23):
+        u = (1 - torch.rand(6, generator=g) * 1e-5).to(device)        # draws from the tail
+        check_draw(x, u, rl.sample_categorical(x, u, top_p=p), top_p=p)

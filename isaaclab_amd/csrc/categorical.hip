@@ -80,8 +80,10 @@ MDP_DEV void finish_row(const EvalArgs& g, const Row<T>& r, int64_t row, float m
     float lp;
     if (a == -1) lp = 0.0f;
     else if (a < 0 || a >= r.V) lp = __builtin_nanf("");
-    else if (!r.allowed((int)a)) lp = s == s ? -kInf : (float)s;
-    else lp = (to_f32(r.x[a]) - m) * inv_t - log_s;
+    else {
+        const float x = r.entry((int)a);               // -inf: masked, or not allowed by itself, also where nothing is (ln s = -inf)
+        lp = x > -kInf || s != s ? (x - m) * inv_t - log_s : -kInf;
+    }
     g.log_prob[row] = lp;
     g.entropy[row] = h;
     if (g.stats) {

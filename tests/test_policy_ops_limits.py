@@ -27,3 +27,21 @@ def test_draw_peaks_over_long_tails(device, vocab):
     for p in (0.9999, 0.99995, 0.99999, 1 - 2.0 ** -23):
         u = (1 - torch.rand(6, generator=g) * 1e-5).to(device)        # draws from the tail
         check_draw(x, u, rl.sample_categorical(x, u, top_p=p), top_p=p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("vocab", [1, 5, 700, 9001])
+def test_evaluation_of_rows_of_minus_infinity(device, dtype, vocab):
+    """A row that holds nothing but -inf where it is allowed: an action in range is one that is not allowed, log_prob -inf, as in
+    a row that a mask empties; entropy and gradient 0."""
+    x = torch.full((5, vocab), -math.inf, dtype=DT[dtype], device=device)
+    a = torch.tensor([0, vocab - 1, vocab // 2, -1, vocab], device=device)
+    one = torch.ones(5, device=device)
+    some = torch.rand(5, vocab, generator=rng_of("allowed", vocab)).to(device) < 0.5
+    behind = torch.where(some, x, torch.zeros_like(x))                 # what is not allowed is finite
+    for y, mask in ((x, None), (x, torch.ones_like(some)), (x, some), (behind, some)):
+        lp, h, grad = run_evaluation(y, a, one, one, mask=mask)
+        check_evaluation(y, a, lp, h, grad, one, one, mask=mask)
+        assert lp[:4].tolist() == [-math.inf] * 3 + [0.0] and bool(lp[4].isnan())
+        assert h.tolist() == [0.0] * 5 and not bool(grad[:4].any())

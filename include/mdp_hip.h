@@ -1273,7 +1273,8 @@ int mdp_categorical_sample(const mdp_categorical_sample_t* args, void* stream);
 
 /* Log-probability of actions[row] and entropy of softmax(logits / temperature) over the allowed entries of every row.
  * Action -1 (a row that had nothing to choose from): log_prob 0; an action that is not allowed: -inf; one outside
- * [-1, vocab): NaN.  A row without allowed entries has entropy 0.  stats (rows, 3), or NULL: what _grad reads.
+ * [-1, vocab): NaN.  A row without allowed entries has entropy 0.  A NaN or +inf among the allowed entries makes a row NaN, and
+ * so does a temperature that is not finite or below 2^-126.  stats (rows, 3), or NULL: what _grad reads.
  * _grad: grad_logits = gradient of sum(grad_log_prob * log_prob + grad_entropy * entropy) by the logits, in their type
  * (either may be NULL: zeros); entries that are not allowed get 0.  Settings, mask and actions as in the forward call. */
 typedef struct {

@@ -42,7 +42,7 @@ struct GradArgs {
 
 MDP_DEV float inverse_temperature(const float* per_row, float scalar, int64_t row) {
     const float t = per_row ? per_row[row] : scalar;
-    return t > 0.0f && t < kInf ? 1.0f / t : __builtin_nanf("");
+    return t >= 1.17549435e-38f && t < kInf ? 1.0f / t : __builtin_nanf("");     // of a denormal it may be infinite
 }
 
 struct Running {

@@ -183,7 +183,7 @@ def evaluate_categorical(logits: torch.Tensor, actions: torch.Tensor, *, tempera
     Action -1 (what a row with nothing allowed was given) has log_prob 0 and no gradient through it, an action that is not
     allowed -inf, one outside [-1, vocab) NaN.  A row with nothing allowed has entropy 0 and gradient 0; entries that are not
     allowed have gradient 0.  A NaN or +inf among the allowed logits makes its row NaN, and so does a per-row temperature that
-    is not positive and finite.
+    is not a finite number of at least 2^-126, the smallest normal one (a temperature for all rows is refused below it).
 
     Inside a captured graph use ``evaluate_categorical_grad``, which does without autograd's own streams and graph nodes."""
     L.require_gpu(logits, "logits")

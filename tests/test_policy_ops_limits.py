@@ -45,3 +45,15 @@ def test_evaluation_of_rows_of_minus_infinity(device, dtype, vocab):
         check_evaluation(y, a, lp, h, grad, one, one, mask=mask)
         assert lp[:4].tolist() == [-math.inf] * 3 + [0.0] and bool(lp[4].isnan())
         assert h.tolist() == [0.0] * 5 and not bool(grad[:4].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [9, 700, 9001])
+def test_evaluation_below_the_smallest_normal_temperature(device, vocab):
+    x = torch.randn(5, vocab, generator=rng_of("none", vocab)).to(device)
+    t = torch.tensor([2.0 ** -127, 1e-39, 1e-45, 0.0, -0.0], device=device)
+    a, one = x.argmax(1), torch.ones(5, device=device)
+    for v in run_evaluation(x, a, one, one, temperature=t):
+        assert bool(v.isnan().all())
+    with pytest.raises(ValueError, match="temperature"):
+        rl.evaluate_categorical(x, a, temperature=2.0 ** -127)

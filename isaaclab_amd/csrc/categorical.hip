@@ -176,11 +176,12 @@ __global__ __launch_bounds__(256) void k_evaluate_long(EvalArgs g) {
 }
 
 // Gradient of an entry: -p (gl + ge (ln p + H)) / T, and + gl / T at the action, with log2 p = (x - m) log2(e) / T - log2 s.
-// Held at or above -300, where p is 0 in 32 bits, an entry that is not allowed gives a zero by itself; only rows that hold a NaN
-// (`whole` false) are told apart entry by entry.
+// Held at or above -300, where p is 0 in 32 bits, an entry that is not allowed gives a zero by itself; only rows that hold a NaN, or
+// whose terms by themselves leave the 32-bit range as 1 / T does near its end (`whole` false), are told apart entry by entry and
+// divided by T last.
 template <typename T>
 struct RowGrad {
-    float m, c, log2_s, a0, a1, hot;
+    float m, c, log2_s, a0, a1, hot, last;              // the last: 1 / T in a row whose other terms are not divided by T
     int action;                                        // -1: none in the row
     bool whole;
     MDP_DEV RowGrad(const GradArgs& g, int64_t row) {
@@ -198,32 +199,42 @@ struct RowGrad {
         hot = gl * inv_t;
         a0 = -(gl + ge * h) * inv_t;
         a1 = -ge * kLn2 * inv_t;
-        whole = a0 - a0 == 0.0f && a1 - a1 == 0.0f && log2_s == log2_s;
+        const float most = fmaf(fabsf(a1), 300.0f, fabsf(a0)) + fabsf(hot);
+        whole = most - most == 0.0f && log2_s == log2_s;
+        last = 1.0f;
+        if (!whole) {
+            hot = gl;
+            a0 = -(gl + ge * h);
+            a1 = -ge * kLn2;
+            last = inv_t;
+        }
     }
     MDP_DEV float operator()(float x) const {
         const float lp = larger(fmaf(x - m, c, -log2_s), -300.0f);
         return __builtin_amdgcn_exp2f(lp) * fmaf(a1, lp, a0);
     }
-    MDP_DEV float of_broken(float x) const {
+    MDP_DEV float by_itself(float x, float own) const {
         if (x == -kInf) return 0.0f;
-        const float lp = fmaf(x - m, c, -log2_s);
-        return __builtin_amdgcn_exp2f(lp) * fmaf(a1, lp, a0);
+        float lp = fmaf(x - m, c, -log2_s);
+        lp = lp < -300.0f ? -300.0f : lp;              // a NaN stays
+        return (__builtin_amdgcn_exp2f(lp) * fmaf(a1, lp, a0) + own) * last;
     }
     // gradients of N entries from entry i0 on, in place
     template <int N>
     MDP_DEV void apply(float (&v)[N], int i0) const {
         const int at = action - i0;
         const bool here = (unsigned)at < (unsigned)N;  // the action is one of them
+        if (!whole) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = by_itself(v[e], here && e == at ? hot : 0.0f);
+            return;
+        }
         uint32_t possible = 0;
         if (here)
 #pragma unroll
             for (int e = 0; e < N; ++e) possible |= e == at && v[e] != -kInf ? 1u << e : 0u;
-        if (whole)
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = (*this)(v[e]);
-        else
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = of_broken(v[e]);
+        for (int e = 0; e < N; ++e) v[e] = (*this)(v[e]);
         if (here)
 #pragma unroll
             for (int e = 0; e < N; ++e) v[e] += possible >> e & 1u ? hot : 0.0f;

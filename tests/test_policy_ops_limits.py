@@ -57,3 +57,76 @@ def test_evaluation_below_the_smallest_normal_temperature(device, vocab):
         assert bool(v.isnan().all())
     with pytest.raises(ValueError, match="temperature"):
         rl.evaluate_categorical(x, a, temperature=2.0 ** -127)
+
+
+def roundings(x, a, lp, h, grad, gl, ge, mask, t, moves):
+    """One row (float64) against its definition, within what the kernels' own roundings allow.  Per entry and unit of U:
+      exponent   (x - max), 1 / T, log2(e) / T (constant and product), their product: 5 |d|, d = (x - max) / T
+      weight     2^x to one step: 2;  sums of a chunk of at most 8: 7;  beyond it in 64 bits;  each change of a thread's largest
+                 entry multiplies what it has by another 2^x: 2 each, at most `moves`
+      s          5 E|d| + 10 + 2 moves (p-weighted mean; the last 1 is its rounding to 32 bits);  ln s: that and 4 of itself (logf)
+      t / s      5 E d^2 + (17 + 2 moves) E|d| + E|d| (what s is off)
+      H          ln s - t / s: both, and 1 of itself
+      log_prob   3 |d_a|, ln s, 1 of itself
+      gradient   p: its exponent 4 |d|, log2 s as ln s and 2 more of itself, 1 of ln p, 2 for 2^x;  gl + ge (ln p + H): ge times what
+                 ln p and H are off, 4 of each term;  1 / T: 1;  gl / T at the action: 2;  the result's own rounding
+    and a tenth more for products of these.  A p below 2^-126 is 0 in 32 bits: what it would give, its terms over T, is lost."""
+    ok = np.ones(len(x), bool) if mask is None else mask
+    want = O.evaluate_row(x, a, mask, t, gl, ge)
+    d = np.where(ok, (x[ok].max() - np.where(ok, x, 0.0)) / t, 0.0)
+    w = np.where(ok, np.exp(-d), 0.0)
+    s = w.sum()
+    p, ln_s = w / s, math.log(s)
+    ln_p = np.where(ok, -d - ln_s, 0.0)
+    mean, square = (p * d).sum(), (p * d * d).sum()
+    off_s = 5 * mean + 10 + 2 * moves
+    off_ln = off_s + 4 * ln_s
+    off_h = off_ln + 5 * square + (17 + 2 * moves) * mean + mean * off_s + abs(want[1])
+    u = 1.1 * U
+    assert abs(lp - want[0]) <= u * (3 * d[a] + off_ln + abs(want[0])) + 1e-30, (lp, want[0])
+    assert abs(h - want[1]) <= u * off_h + 1e-30, (h, want[1])
+    off_lnp = 4 * d + off_ln + 2 * ln_s + np.abs(ln_p)
+    terms = abs(gl) + abs(ge) * (np.abs(ln_p) + abs(want[1]))
+    tol = p * ((off_lnp + 2) * np.abs(gl + ge * (ln_p + want[1])) + abs(ge) * (off_lnp + off_h) + 5 * terms) * u / t
+    tol[a] += 2 * u * abs(gl) / t
+    tol += 2.0 ** -126 * terms / t
+    return want, tol
+
+
+def check_roundings(x, a, lp, h, grad, gl, ge, mask=None, temperature=1.0, moves=0):
+    step = torch.finfo(grad.dtype).eps / 2
+    floor = torch.finfo(grad.dtype).smallest_normal * torch.finfo(grad.dtype).eps / 2
+    xs, gs, lps, hs, gls, ges = f64(x), f64(grad), f64(lp), f64(h), f64(gl), f64(ge)
+    for r in range(len(xs)):
+        want, tol = roundings(xs[r], int(a[r]), lps[r], hs[r], gs[r], gls[r], ges[r],
+                              None if mask is None else mask[r].cpu().numpy(),
+                              f64(temperature)[r] if isinstance(temperature, torch.Tensor) else f32v(temperature), moves)
+        tol = tol + step * np.abs(want[2]) * 1.01 + floor
+        err = np.abs(gs[r] - want[2])
+        assert (err <= tol).all(), (r, err.max(), tol[(err - tol).argmax()])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [9, 700, 9001])
+def test_evaluation_at_the_smallest_temperatures(device, dtype, vocab):
+    """Down to the smallest normal number the definition holds, with logits that lie as near to each other: gradients are of the
+    order of 1 / T, and 0 where the probability is.  Below it, as for a single number, a temperature is none: NaN."""
+    g = rng_of("cold evaluation", dtype, vocab)
+    t = torch.tensor([2.0 ** -126, 1.2e-38, 2e-38, 1e-37, 1e-36, 1e-30])
+    x = (-torch.rand(6, vocab, generator=g) * 2000 * t[:, None]).to(DT[dtype])
+    a = torch.randint(0, vocab, (6,), generator=g)
+    a[::2] = x.float().argmax(1)[::2]
+    gl, ge = (torch.rand(6, generator=g) * 2 - 1 for _ in range(2))
+    x, a, gl, ge, t = (v.to(device) for v in (x, a, gl, ge, t))
+    moves = 0 if vocab < 1000 else 6
+    check_roundings(x, a, *run_evaluation(x, a, gl, ge, temperature=t), gl, ge, temperature=t, moves=moves)
+    mask = torch.rand(6, vocab, generator=g).to(device) < 0.7
+    mask.scatter_(1, a[:, None], True)
+    check_roundings(x, a, *run_evaluation(x, a, gl, ge, temperature=t, mask=mask), gl, ge, mask=mask, temperature=t, moves=moves)
+    # an action that is certain: nothing is left of a gradient whose terms are beyond float32
+    sure = torch.full((2, vocab), -1.0, dtype=DT[dtype], device=device)
+    sure[:, 3] = 1.0
+    three, five = torch.full((2,), 3, device=device), torch.tensor([5.0, -40.0], device=device)
+    lp, h, grad = run_evaluation(sure, three, five, five, temperature=t[:2])
+    assert not bool(lp.any()) and not bool(h.any()) and not bool(grad.any())

@@ -60,7 +60,7 @@ def _setting(value, name: str, dtype: torch.dtype, logits: torch.Tensor, low: fl
         raise ValueError(f"{name} gets no gradient: pass it detached")
     lead = logits.shape[:-1]
     if dtype == torch.int32 and value.dtype != dtype:
-        value = value.clamp(-1, 2147483647)
+        value = value.to(torch.int64).clamp(-1, 2147483647)            # the narrower types hold no such bounds
     try:
         return value.detach().to(dtype).expand(lead).contiguous(), 0.0
     except RuntimeError:

@@ -130,3 +130,12 @@ def test_evaluation_at_the_smallest_temperatures(device, dtype, vocab):
     three, five = torch.full((2,), 3, device=device), torch.tensor([5.0, -40.0], device=device)
     lp, h, grad = run_evaluation(sure, three, five, five, temperature=t[:2])
     assert not bool(lp.any()) and not bool(h.any()) and not bool(grad.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8, torch.uint16, torch.uint32, torch.bool])
+def test_draw_top_k_of_any_integer_type(device, kind):
+    g = rng_of("kinds")
+    x, u = torch.randn(5, 300, generator=g).to(device), torch.rand(5, generator=g).to(device)
+    k = torch.tensor([0, 1, 3, 7, 120]).to(kind)
+    check_draw(x, u, rl.sample_categorical(x, u, top_k=k.to(device)), top_k=k.to(torch.int64))

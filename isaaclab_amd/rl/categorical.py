@@ -59,6 +59,8 @@ def _setting(value, name: str, dtype: torch.dtype, logits: torch.Tensor, low: fl
     if value.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} gets no gradient: pass it detached")
     lead = logits.shape[:-1]
+    if dtype == torch.int32 and (value.is_floating_point() or value.is_complex()):
+        raise ValueError(f"{name} must be of whole numbers, an integer tensor, got {value.dtype}")
     if dtype == torch.int32 and value.dtype != dtype:
         value = value.to(torch.int64).clamp(-1, 2147483647)            # the narrower types hold no such bounds
     try:
@@ -91,10 +93,11 @@ def sample_categorical(logits: torch.Tensor, u: torch.Tensor | None = None, *, t
     the device generator of ``isaaclab_amd.utils.math`` (``seed_samplers``; seeded, or drawn from, before a capture), fresh on
     every replay of a captured call.
 
-    Kept are the ``top_k`` largest allowed logits (0: all; equal ones by lowest index), of these the fewest largest that hold a
-    share ``top_p`` of their weight (one at least), of these the ones of at least ``min_p`` times the largest weight.
-    ``temperature`` 0 (or below the smallest normal float) takes the largest logit (the first of equal ones) with log_prob 0.  ``log_prob`` is that of the
-    distribution drawn from: without ``top_k`` / ``top_p`` / ``min_p`` it is what ``evaluate_categorical`` says.
+    Kept are the ``top_k`` largest allowed logits (0: all; equal ones by lowest index; per row: an integer tensor, what is
+    negative counts as 0), of these the fewest largest that hold a share ``top_p`` of their weight (one at least), of these the
+    ones of at least ``min_p`` times the largest weight.  ``temperature`` 0 (or below the smallest normal float) takes the largest
+    logit (the first of equal ones) with log_prob 0.  ``log_prob`` is that of the distribution drawn from: without ``top_k`` /
+    ``top_p`` / ``min_p`` it is what ``evaluate_categorical`` says.
 
     A row in which nothing is allowed gives action -1 and log_prob 0; a row with a NaN or +inf among its allowed logits gives
     action -1 and log_prob NaN, and so does a per-row temperature that is negative or NaN.  A per-row ``top_p`` / ``min_p`` that is

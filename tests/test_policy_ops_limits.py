@@ -139,3 +139,12 @@ def test_draw_top_k_of_any_integer_type(device, kind):
     x, u = torch.randn(5, 300, generator=g).to(device), torch.rand(5, generator=g).to(device)
     k = torch.tensor([0, 1, 3, 7, 120]).to(kind)
     check_draw(x, u, rl.sample_categorical(x, u, top_k=k.to(device)), top_k=k.to(torch.int64))
+
+
+@pytest.mark.gpu
+def test_draw_refuses_fractions_of_entries(device):
+    """A top_k for each row is of whole numbers, as the one for all rows: their type says so."""
+    x, u = torch.zeros(2, 3, device=device), torch.zeros(2, device=device)
+    for k in (torch.tensor([2.5, 1.0], device=device), torch.ones(2, dtype=torch.bfloat16, device=device)):
+        with pytest.raises(ValueError, match="whole number"):
+            rl.sample_categorical(x, u, top_k=k)

@@ -32,6 +32,12 @@ struct Settings {
     MDP_DEV double weight(float x, float m) const { return exp2_neg(((double)x - (double)m) * c); }
 };
 
+// ln(w / mass), w the weight of x: from x itself where w is a denormal or near one and holds fewer bits than the result
+constexpr double kLight = 1e-290;
+MDP_DEV float log_share_of_light(float x, float m, double c, double mass) {
+    return (float)(((double)x - (double)m) * c * 0.6931471805599453 - log(mass));
+}
+
 // an entry as a word that rises in the order (value falling, place rising)
 MDP_DEV uint64_t word_of(float x, int place) { return (uint64_t)(~key_of(x)) << 32 | (uint32_t)place; }
 MDP_DEV float value_of(uint64_t word) { return of_key(~(uint32_t)(word >> 32)); }
@@ -352,6 +358,13 @@ __global__ __launch_bounds__(G > 64 ? G : 256, 4) void k_sample_short(SampleArgs
     }
     g.actions[mine] = q.good ? found : -1;
     g.log_prob[mine] = q.good ? (float)log(found_w / mass) : broken ? __builtin_nanf("") : 0.0f;
+    if (__builtin_expect(q.good && found_w < kLight, 0)) {      // all that it takes is read again, and kept in no register until here
+        const Row<T> again(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, mine);
+        float top = -kInf;
+#pragma unroll 1
+        for (int i = 0; i < again.V; ++i) top = larger(again.entry(i), top);
+        g.log_prob[mine] = log_share_of_light(again.entry(found), top, Settings(g, mine).c, mass);
+    }
 }
 
 // Longer rows: a block a row.  Each wave owns a contiguous piece of the row, so that running sums follow the index; of it every
@@ -819,6 +832,7 @@ struct LongRow {
             }
         }
         answer(g, row, found, found_w, total);
+        if (found_w < kLight) g.log_prob[row] = log_share_of_light(r.entry(found), m, s.c, total);     // the list's entries are heavier
     }
 };
 

@@ -148,3 +148,22 @@ def test_draw_refuses_fractions_of_entries(device):
     for k in (torch.tensor([2.5, 1.0], device=device), torch.ones(2, dtype=torch.bfloat16, device=device)):
         with pytest.raises(ValueError, match="whole number"):
             rl.sample_categorical(x, u, top_k=k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [3, 200, 700, 3000, 9000, 40000])
+def test_draw_of_the_smallest_weights(device, vocab):
+    """u = 0 draws the first kept entry, however light: its log-probability keeps 32 bits where its weight, below 2^-1022, does not."""
+    d = torch.tensor([-700.0, -708.0, -712.3, -725.1, -735.0, -743.0])
+    x = torch.full((6, vocab), -2000.0)
+    x[:, 1] = d
+    x[:, vocab - 1] = 0.0
+    x, u = x.to(device), torch.zeros(6, device=device)
+    for s in (dict(), dict(top_k=2), dict(temperature=0.5)):
+        t = s.get("temperature", 1.0)
+        a, lp = rl.sample_categorical(x * t, u, **s)
+        assert a.tolist() == [1] * 6
+        np.testing.assert_allclose(f64(lp), f64(x[:, 1]), rtol=2 * U)              # ln(1 + e^-700) is 0
+    x[:, 0] = math.nan
+    a, lp = rl.sample_categorical(x, u)
+    assert a.tolist() == [-1] * 6 and bool(lp.isnan().all())

@@ -1292,7 +1292,7 @@ int mdp_categorical_evaluate_grad(const mdp_categorical_eval_t* args, const floa
 
 /* The norm of many gradients taken as one vector, and clipping to it.  `grads` is a HOST array (read during the call) of dense
  * device tensors.  norm_kind: 2 = root of the sum of squares, 1 = sum of magnitudes, 0 = largest magnitude (inf norm); sums
- * and squares in 64 bits, in an order that depends on the sizes alone.
+ * and squares in 64 bits, in an order that depends on the sizes and element types alone.
  * mdp_grad_norm:  *norm (device float).
  * mdp_grad_clip:  the same, then out = grad * min(1, max_norm / (norm + 1e-6)) for every tensor; out may be grad itself (left
  * untouched where nothing is clipped) or another tensor of the same type or float32.  A norm that is infinite makes the factor

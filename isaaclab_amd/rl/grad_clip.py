@@ -1,5 +1,6 @@
 """The norm of many gradients taken as one vector, and clipping to it (``mdp_grad_norm`` / ``mdp_grad_clip``): float32,
-bfloat16 and float16 tensors in one call, sums in 64 bits in an order that depends on the sizes alone, no synchronisation."""
+bfloat16 and float16 tensors in one call, sums in 64 bits in an order that depends on the sizes and element types alone, no
+synchronisation."""
 from __future__ import annotations
 
 from array import array

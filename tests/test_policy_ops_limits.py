@@ -167,3 +167,25 @@ def test_draw_of_the_smallest_weights(device, vocab):
     x[:, 0] = math.nan
     a, lp = rl.sample_categorical(x, u)
     assert a.tolist() == [-1] * 6 and bool(lp.isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_grad_sums_do_not_depend_on_the_address(device, dtype, kind):
+    """The same values behind an odd offset give the same partial sums, bit for bit."""
+    n = 5 * 4096 + 77
+    x = (torch.randn(n, generator=rng_of("address", dtype)) * 0.1).to(DT[dtype]).to(device)
+    sums = []
+    for shift in range(9):
+        base = torch.zeros(n + 16, dtype=DT[dtype], device=device)
+        y = base[shift:shift + n].copy_(x)
+        work = torch.zeros(L.lib.mdp_grad_workspace(1), dtype=torch.float64, device=device)
+        norm = torch.zeros((), device=device)
+        table = (L.MdpGrad * 1)(L.MdpGrad(y.data_ptr(), None, n, L.DTYPES[y.dtype], 0))
+        L.launch(L.lib.mdp_grad_norm, 0, table, 1, kind, work.data_ptr(), norm.data_ptr())
+        sums.append(work[:7].clone())                   # six partial sums and what they join to
+    want = f64(x)
+    want = np.abs(want).max() if kind == 0 else np.abs(want).sum() if kind == 1 else (want ** 2).sum()
+    np.testing.assert_allclose(sums[0][6].item(), want, rtol=n * 2.0 ** -53)
+    assert all(torch.equal(s, sums[0]) for s in sums[1:])

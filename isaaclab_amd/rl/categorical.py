@@ -200,8 +200,8 @@ def evaluate_categorical_grad(logits: torch.Tensor, actions: torch.Tensor, grad_
                               grad_entropy: torch.Tensor | None, *, temperature=1.0,
                               mask: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(log_prob, entropy, grad_logits)``: the evaluation and the gradient of ``sum(grad_log_prob * log_prob + grad_entropy
-    * entropy)`` by the logits, in their type, without autograd (two launches that a graph may capture).  ``grad_*``: float32,
-    leading shape, or None for zeros."""
+    * entropy)`` by the logits, in their type, without autograd (two launches that a graph may capture): what goes in may
+    require a gradient, none of the results does or passes one on.  ``grad_*``: float32, leading shape, or None for zeros."""
     x, ld = _logit_rows(logits.detach() if isinstance(logits, torch.Tensor) else logits)
     actions = _per_row(actions, "actions", torch.int64, logits)
     m, ld_mask = _mask_rows(mask, logits)

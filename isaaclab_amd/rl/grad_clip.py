@@ -133,7 +133,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> tupl
     """``(out, norm)``: like ``clip_grad_norm_`` on the tensors ``grads`` with the result in ``out``, one tensor for each
     gradient, of its type or float32 (16-bit gradients clipped into the 32-bit ones that an optimiser reads); new tensors of
     the gradients' types when omitted.  An ``out`` may be its gradient itself; otherwise outputs and gradients must not
-    overlap."""
+    overlap.  Works on values, as every function here: nothing is recorded for autograd, whatever requires a gradient."""
     grads = _as_list(grads)
     if out is None:
         out = [torch.empty_like(_known(g)) for g in grads]

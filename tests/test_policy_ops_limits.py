@@ -189,3 +189,18 @@ def test_grad_sums_do_not_depend_on_the_address(device, dtype, kind):
     want = np.abs(want).max() if kind == 0 else np.abs(want).sum() if kind == 1 else (want ** 2).sum()
     np.testing.assert_allclose(sums[0][6].item(), want, rtol=n * 2.0 ** -53)
     assert all(torch.equal(s, sums[0]) for s in sums[1:])
+
+
+@pytest.mark.gpu
+def test_results_outside_autograd(device):
+    """evaluate_categorical_grad and clip_grads work on values: what they are given may require a gradient, what they give has none."""
+    g = rng_of("outside")
+    x = torch.randn(4, 30, generator=g).to(device).requires_grad_()
+    a = torch.randint(0, 30, (4,), generator=g).to(device)
+    gl, ge = (torch.randn(4, generator=g).to(device).requires_grad_() for _ in range(2))
+    got = rl.evaluate_categorical_grad(x, a, gl, ge)
+    out, norm = rl.clip_grads([x], 0.5)
+    for p, q in zip(got, rl.evaluate_categorical_grad(x.detach(), a, gl.detach(), ge.detach())):
+        assert not p.requires_grad and torch.equal(p, q)
+    assert not norm.requires_grad and not out[0].requires_grad
+    assert torch.equal(out[0], rl.clip_grads([x.detach()], 0.5)[0][0])

@@ -1296,7 +1296,7 @@ int mdp_categorical_evaluate_grad(const mdp_categorical_eval_t* args, const floa
  * mdp_grad_norm:  *norm (device float).
  * mdp_grad_clip:  the same, then out = grad * min(1, max_norm / (norm + 1e-6)) for every tensor; out may be grad itself (left
  * untouched where nothing is clipped) or another tensor of the same type or float32.  A norm that is infinite makes the factor
- * 0, one that is NaN makes it NaN.  Outputs overlap neither each other nor another tensor's gradient (MDP_ERR_INVALID).
+ * 0 (NaN where max_norm is infinite too), one that is NaN makes it NaN.  Outputs overlap neither each other nor another tensor's gradient (MDP_ERR_INVALID).
  * workspace: mdp_grad_workspace(n) doubles, not shared by calls that may run at the same time; NULL is refused. */
 typedef struct {
     const void* grad; void* out; int64_t count; int32_t dtype; int32_t out_dtype;

@@ -121,7 +121,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0) -> torc
     counts once) in place by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm before (float32, on the device).
 
     The factor is rounded to 32 bits and every product once to its gradient's type.  A norm that is infinite makes the factor
-    0, one that is NaN makes every gradient NaN; nothing synchronises to look."""
+    0, or NaN where ``max_norm`` is infinite too; one that is NaN makes every gradient NaN; nothing synchronises to look."""
     grads = [p.grad for p in dict.fromkeys(_as_list(parameters)) if p.grad is not None]
     norm = _launch(grads, None, _kind(norm_type), _bound(max_norm))
     if grads:

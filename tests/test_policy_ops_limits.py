@@ -204,3 +204,15 @@ def test_results_outside_autograd(device):
         assert not p.requires_grad and torch.equal(p, q)
     assert not norm.requires_grad and not out[0].requires_grad
     assert torch.equal(out[0], rl.clip_grads([x.detach()], 0.5)[0][0])
+
+
+@pytest.mark.gpu
+def test_clip_with_an_infinite_bound(device):
+    """An infinite bound measures the norm and leaves finite gradients as they are; over an infinite norm it is no number."""
+    x = torch.randn(5000, generator=rng_of("unbounded")).to(device)
+    out, norm = rl.clip_grads([x], math.inf)
+    assert torch.equal(out[0], x) and bool(norm.isfinite())
+    y = x.clone()
+    y[77] = math.inf
+    out, norm = rl.clip_grads([y], math.inf)
+    assert float(norm) == math.inf and bool(out[0].isnan().all())

@@ -216,3 +216,21 @@ def test_clip_with_an_infinite_bound(device):
     y[77] = math.inf
     out, norm = rl.clip_grads([y], math.inf)
     assert float(norm) == math.inf and bool(out[0].isnan().all())
+
+
+@pytest.mark.gpu
+def test_ratio_of_an_unchanged_policy(device):
+    """What is drawn uncut, with the temperature and the mask that it is evaluated with, has the ratio 1: the documented update.  A
+    draw that top_p cuts has the log-probability of what is left, so the ratio is the kept mass."""
+    g = rng_of("ratio")
+    logits = (torch.randn(64, 12, 33, generator=g) * 2).to(device)
+    allowed = torch.rand(64, 12, 33, generator=g).to(device) < 0.8
+    u = torch.rand(64, 12, generator=g).to(device)
+    actions, old = rl.sample_categorical(logits, u, temperature=0.9, mask=allowed)
+    log_prob, _ = rl.evaluate_categorical(logits, actions, temperature=0.9, mask=allowed)
+    # three roundings of d = (x - max) / T below 2 * 9 / 0.9, and the sum's: see test_evaluation_within_its_roundings
+    np.testing.assert_allclose(f64(log_prob - old), 0.0, atol=U * 250)
+    actions, old = rl.sample_categorical(logits, u, temperature=0.9, top_p=0.7, mask=allowed)
+    log_prob, _ = rl.evaluate_categorical(logits, actions, temperature=0.9, mask=allowed)
+    ratio = f64(torch.exp(log_prob - old))
+    assert ratio.min() >= f32v(0.7) - 1e-5 and (ratio < 1.0).mean() > 0.9

@@ -234,3 +234,45 @@ def test_ratio_of_an_unchanged_policy(device):
     log_prob, _ = rl.evaluate_categorical(logits, actions, temperature=0.9, mask=allowed)
     ratio = f64(torch.exp(log_prob - old))
     assert ratio.min() >= f32v(0.7) - 1e-5 and (ratio < 1.0).mean() > 0.9
+
+
+LARGE = [dict(), dict(top_p=0.9), dict(top_k=50, top_p=0.8, temperature=0.7), dict(min_p=0.05), dict(top_k=200),
+         dict(top_p=0.99, temperature=3.0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype, vocab", [("f32", 4101), ("f32", 16380), ("bf16", 8203), ("bf16", 32001), ("f16", 9000), ("f16", 32750)])
+def test_draw_large_batches_of_long_rows(device, dtype, vocab, masked):
+    """512 rows and more of 1025 to 4096 chunks are drawn by blocks of 256 threads."""
+    g = rng_of("many long", dtype, vocab)
+    rows = 515
+    x = (torch.randn(rows, vocab, generator=g) * torch.rand(rows, 1, generator=g) * 4).to(DT[dtype]).to(device)
+    u = torch.rand(rows, generator=g).to(device)
+    mask = (torch.rand(rows, vocab, generator=g) < torch.rand(rows, 1, generator=g)).to(device) if masked else None
+    pick = torch.cat([torch.arange(0, rows, 41), torch.tensor([1, rows - 1])]).to(device)
+    per_row = dict(temperature=(torch.rand(rows, generator=g) * 2).to(device), top_k=torch.randint(0, 300, (rows,), generator=g).to(device),
+                   top_p=(torch.rand(rows, generator=g) * 1.2).to(device))
+    for s in LARGE + [per_row]:
+        a, lp = rl.sample_categorical(x, u, mask=mask, **s)
+        part = {k: v[pick] if isinstance(v, torch.Tensor) else v for k, v in s.items()}
+        check_draw(x[pick], u[pick], (a[pick], lp[pick]), mask=None if mask is None else mask[pick], **part)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, vocab", [("f32", 16390), ("f32", 70001), ("bf16", 32771), ("bf16", 140003), ("f16", 50001)])
+def test_draw_longest_rows_with_masks(device, dtype, vocab):
+    """Rows of more than 4096 chunks, masked: at random, all but a few, everything, at the chunks' edges."""
+    g = rng_of("long masked", dtype, vocab)
+    x = (torch.randn(7, vocab, generator=g) * 2).to(DT[dtype])
+    mask = torch.rand(7, vocab, generator=g) < torch.tensor([0.7, 0.01, 0.5, 0.5, 1.0, 0.0, 0.9])[:, None]
+    mask[3, :vocab // 2] = False
+    mask[4, ::8] = False
+    x[2, ~mask[2]] = math.nan
+    x, mask = x.to(device), mask.to(device)
+    u = torch.rand(7, generator=g).to(device)
+    wide = torch.zeros(7, vocab + 3, dtype=torch.bool, device=device)
+    wide[:, 3:] = mask                                   # the same at an odd offset
+    for s in LARGE:
+        for m in (mask, wide[:, 3:]):
+            check_draw(x, u, rl.sample_categorical(x, u, mask=m, **s), mask=m, **s)

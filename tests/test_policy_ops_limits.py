@@ -276,3 +276,56 @@ def test_draw_longest_rows_with_masks(device, dtype, vocab):
     for s in LARGE:
         for m in (mask, wide[:, 3:]):
             check_draw(x, u, rl.sample_categorical(x, u, mask=m, **s), mask=m, **s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("vocab", [2, 19, 64, 255, 1024, 2050, 5003, 33001, 131075, 1000003])
+def test_evaluation_within_its_roundings(device, dtype, vocab):
+    """A thread's largest entry changes at most once in 1024 chunks, once at the row's edges and once when the waves join."""
+    g = rng_of("roundings", dtype, vocab)
+    chunk = 128 // torch.finfo(DT[dtype]).bits
+    moves = 0 if vocab <= 512 * chunk - chunk else vocab // (1024 * chunk) + 3
+    for n, t in enumerate((1.0, 0.6, 2.5)):
+        rows = 16 if vocab < 3000 else 2
+        x = (torch.randn(rows, vocab, generator=g) * (0.5, 3.0, 8.0)[n]).to(DT[dtype]).to(device)
+        a = torch.randint(0, vocab, (rows,), generator=g).to(device)
+        gl, ge = (torch.randn(rows, generator=g).to(device) for _ in range(2))
+        check_roundings(x, a, *run_evaluation(x, a, gl, ge, temperature=t), gl, ge, temperature=t, moves=moves)
+        mask = torch.rand(rows, vocab, generator=g).to(device) < 0.6
+        mask.scatter_(1, a[:, None], True)
+        check_roundings(x, a, *run_evaluation(x, a, gl, ge, temperature=t, mask=mask), gl, ge, mask=mask, temperature=t, moves=moves)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_evaluation_sums_what_32_bits_would_lose(device, dtype):
+    """8192 large entries, then four million that weigh 7e-8 to 1.5e-8 of one each: 584 to 130 U of the sum, which a thread that added
+    them up one by one in 32 bits, 32 large ones first, would lose; the tolerance is about 60 U.  No thread's largest entry changes
+    behind its first."""
+    vocab, first = (1 << 22) + 5, 8192
+    x = torch.zeros(3, vocab, dtype=DT[dtype])
+    for r, low in enumerate((-16.5, -17.25, -18.0)):
+        x[r, first:] = low
+    x = x.to(device)
+    a = torch.tensor([0, first, vocab - 1], device=device)
+    gl, ge = torch.tensor([1.0, -2.0, 0.5], device=device), torch.tensor([0.5, 1.0, -1.0], device=device)
+    check_roundings(x, a, *run_evaluation(x, a, gl, ge), gl, ge)
+
+
+@pytest.mark.gpu
+def test_gradient_of_a_very_long_flat_row(device):
+    """3.3e7 equal entries: gl (delta - 1 / V); the entropy of a flat row is at its maximum, its gradient 0.  Its two terms, ln p and
+    H = ln V, cancel within their roundings: 4 ln V of ln s, 2 and 1 more of it, 12 of the sum, in either, and 4 of each product."""
+    vocab = (1 << 25) + 77
+    x = torch.zeros(1, vocab, device=device)
+    gl, ge = torch.tensor([3.0], device=device), torch.tensor([-2.0], device=device)
+    for at in (0, 12345, vocab - 1):
+        a = torch.tensor([at], device=device)
+        lp, h, grad = rl.evaluate_categorical_grad(x, a, gl, ge)
+        ln = math.log(vocab)
+        tol = U / vocab * (3.0 * (7 * ln + 20) + 2.0 * (2 * (7 * ln + 20) + 8 * ln))
+        rest = f64(grad)[0]
+        assert abs(rest[at] - 3.0 * (1 - 1 / vocab)) <= tol + 3 * 2 * U
+        rest = np.delete(rest, at)
+        assert np.abs(rest + 3.0 / vocab).max() <= tol

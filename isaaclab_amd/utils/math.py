@@ -315,8 +315,18 @@ def seed_samplers(seed: int, device="cuda:0") -> None:
     """Explicit seed of the device generator of ``device`` (stays until the next call of this function)."""
     dev = torch.device(device)
     idx = L.device_index(dev)
-    _sampler_state[idx] = torch.tensor([int(seed) & 0x7FFFFFFFFFFFFFFF, 0], dtype=torch.int64, device=dev)
+    _set_state(idx, dev, seed)
     _sampler_seed[idx] = None
+
+
+def _set_state(idx: int, dev: torch.device, seed: int) -> None:
+    """In place where there is a state: the launches of captured graphs read and advance the memory that they were captured with."""
+    state = torch.tensor([int(seed) & 0x7FFFFFFFFFFFFFFF, 0], dtype=torch.int64)
+    if idx in _sampler_state:
+        with torch.inference_mode():                    # also where the first draw was made in inference mode
+            _sampler_state[idx].copy_(state)
+    else:
+        _sampler_state[idx] = state.to(dev)
 
 
 def _state(device) -> torch.Tensor:
@@ -331,7 +341,7 @@ def _state(device) -> torch.Tensor:
     # starts a new stream (the state is rebuilt when torch.initial_seed() no longer is the seed it was derived from)
     seed_now = torch.initial_seed()
     if idx not in _sampler_state or (_sampler_seed.get(idx) is not None and _sampler_seed[idx] != seed_now):
-        _sampler_state[idx] = torch.tensor([int(seed_now) & 0x7FFFFFFFFFFFFFFF, 0], dtype=torch.int64, device=dev)
+        _set_state(idx, dev, seed_now)
         _sampler_seed[idx] = seed_now
     return _sampler_state[idx]
 

@@ -329,3 +329,43 @@ def test_gradient_of_a_very_long_flat_row(device):
         assert abs(rest[at] - 3.0 * (1 - 1 / vocab)) <= tol + 3 * 2 * U
         rest = np.delete(rest, at)
         assert np.abs(rest + 3.0 / vocab).max() <= tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", ["seed_samplers", "manual_seed"])
+def test_seeding_behind_a_capture(device, seed):
+    """A captured draw goes on with the device's generator, whatever it is seeded with later, and writes to nothing else."""
+    from isaaclab_amd.utils import math as M
+
+    x = torch.zeros(5000, 50, device=device)
+    M.seed_samplers(5, device)
+
+    def reseed(n):
+        if seed == "seed_samplers":
+            return M.seed_samplers(n, device)
+        M._sampler_seed[0] = -1                         # a state that follows torch's seed, as it does until seed_samplers
+        torch.manual_seed(n)
+
+    reseed(6)
+    rl.sample_categorical(x)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        out = rl.sample_categorical(x)[0]
+    reseed(7)
+    eager = [rl.sample_categorical(x)[0] for _ in range(3)]
+    reseed(7)
+    first = rl.sample_categorical(x)[0]
+    others = [torch.zeros(2, dtype=torch.int64, device=device) for _ in range(64)]       # where a state might have been
+    assert torch.equal(first, eager[0])
+    for n in (1, 2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[n])
+    assert not any(bool(t.any()) for t in others)
+    with torch.inference_mode():
+        reseed(8)
+        inside = rl.sample_categorical(x)[0]
+    reseed(8)
+    assert torch.equal(rl.sample_categorical(x)[0], inside)
+    M.seed_samplers(1, device)

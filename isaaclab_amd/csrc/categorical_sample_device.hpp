@@ -62,10 +62,11 @@ MDP_DEV void wave_sync() {
 // Rows of up to G K chunks, 16 entries a lane: G lanes of a wave, or a block of G = 128 or 256, hold a row and its weights in
 // registers.  Groups of a wave go through their loops together until the last is done.
 //
-// Bound by instructions: 49152 x 256 float32 with top_p takes 44 us, 1730 vector instructions for a wave's four rows (300 of them the
-// weights), where the 50 MB are 11 us at the copy rate; uncut it takes 20.  Searching the border by halving the value range, sixteen
-// compares and 64-bit adds a step, took 71.  The registers that hold entries and weights leave four waves a SIMD; with five (96
-// registers) what spills costs more: 53.
+// Bound by instructions: 49152 x 256 float32 with top_p takes 46 us, 1700 vector instructions for a wave's four rows (300 of them the
+// weights), where the 50 MB are 11 us at the copy rate; uncut it takes 22.  Searching the border by halving the value range, sixteen
+// compares and 64-bit adds a step, took 71 where this took 44.  Entries and weights leave four waves a SIMD, and their 128 registers
+// do not hold all: 11 to 42 are spilled (2 or 3 where 256 lanes hold 16-bit rows), most of them by rows of up to 64 entries.  With five
+// waves (96 registers) what spills costs more: 53.
 template <typename T, int G, int K>
 struct ShortRow {
     static constexpr int N = Chunk<T>::N, size = G, capacity = G;
@@ -947,8 +948,8 @@ void launch_sample(const SampleArgs& g, hipStream_t s) {
     }
     SHORT(4) SHORT(8) SHORT(16) SHORT(32) SHORT(64)
     // From here to 4096 entries a row fits the registers of a block just as well; only a small top_k is quicker by the list of
-    // candidates (float32, 2^26 entries in rows of 1028 / 2048 / 4096: top_p 452 / 250 / 331 us against 1130 / 590 / 433 by list and
-    // whole row, top_k 40 402 / 214 / 241 against 273 / 144 / 90).
+    // candidates (float32, 2^26 entries in rows of 1028 / 2048 / 4096: top_p 411 / 223 / 233 us against 1130 / 590 / 433 by list and
+    // whole row, top_k 40 388 / 199 / 207 against 272 / 144 / 90).
     const bool few = !g.top_k && g.top_k_s > 0 && g.top_k_s <= 64;
     if (!few) { SHORT(128) SHORT(256) }
 #undef SHORT
@@ -962,8 +963,8 @@ void launch_sample(const SampleArgs& g, hipStream_t s) {
         hipLaunchKernelGGL((k_sample_whole<T, MASK, THREADS, 0, true>), grid, dim3(THREADS), 0, s, g);                          \
     }
     // Four blocks of 256 threads on a CU work on four rows in turn, one of 1024 on one: with many rows the former hide each other's
-    // waits (bfloat16 rows of 32000, top_p: 1024 of them 169 us against 216), with fewer than two a CU the latter is done sooner (256
-    // of them 59 us against 83).
+    // waits (bfloat16 rows of 32000, top_p: 1024 of them 164 us against 216), with fewer than two a CU the latter is done sooner (256
+    // of them 55 us against 83).
     if (chunks <= 256 * 4) { LONG(256, 4) }
     else if (chunks <= 256 * 16 && g.rows >= 512) { LONG(256, 16) }
     else if (chunks <= 1024 * 4) { LONG(1024, 4) }

@@ -2,8 +2,9 @@
 
 Both work on the last axis of ``logits`` (float32, bfloat16 or float16; any leading axes; rows may have any stride) with an
 optional boolean ``mask`` of the allowed entries that broadcasts against it, and with settings that are numbers or tensors
-that broadcast against the leading axes (one per row).  One launch each (``mdp_categorical_*``) on the current stream of the
-logits' device; sums of a draw are in 64 bits."""
+that broadcast against the leading axes (one per row).  On the current stream of the logits' device, one launch each
+(``mdp_categorical_*``), two for a draw of long rows that settings cut, one more where it draws from the generator; sums of a
+draw are in 64 bits."""
 from __future__ import annotations
 
 import torch
@@ -91,7 +92,7 @@ def sample_categorical(logits: torch.Tensor, u: torch.Tensor | None = None, *, t
     ``u`` (float32, leading shape, in [0, 1)) makes the draw: the answer is the first kept entry, by index, up to which the
     kept entries hold more than a share ``u`` of their weight ``exp(logit / temperature)``.  Without it the numbers come from
     the device generator of ``isaaclab_amd.utils.math`` (``seed_samplers``; seeded, or drawn from, before a capture), fresh on
-    every replay of a captured call.
+    every replay of a captured call; there is one for each device, so calls that draw from it on two streams have to be ordered.
 
     Kept are the ``top_k`` largest allowed logits (0: all; equal ones by lowest index; per row: an integer tensor, what is
     negative counts as 0), of these the fewest largest that hold a share ``top_p`` of their weight (one at least), of these the

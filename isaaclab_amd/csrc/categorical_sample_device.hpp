@@ -14,16 +14,16 @@ constexpr uint32_t kStream = 0x43415447u;
 struct Settings {
     double c;                                          // log2(e) / T; a NaN for a temperature that is negative or NaN
     int k;                                             // 0: no limit
-    double p, mp;                                      // p = 1, mp = 0: no limit
+    float p, mp;                                       // p = 1, mp = 0: no limit
     double u;
     MDP_DEV Settings(const SampleArgs& g, int64_t row) {
         k = g.top_k ? g.top_k[row] : g.top_k_s;
         float pf = g.top_p ? g.top_p[row] : g.top_p_s, mf = g.min_p ? g.min_p[row] : g.min_p_s;
         if (k < 0) k = 0;
-        p = pf < 1.0f ? (pf > 0.0f ? (double)pf : 0.0) : 1.0;
-        mp = mf > 0.0f ? (mf < 1.0f ? (double)mf : 1.0) : 0.0;
+        p = pf < 1.0f ? (pf > 0.0f ? pf : 0.0f) : 1.0f;
+        mp = mf > 0.0f ? (mf < 1.0f ? mf : 1.0f) : 0.0f;
         c = g.temperature ? rate_of(g.temperature[row]) : g.rate;
-        if (c == kGreedy) { k = 1; p = 1.0; mp = 0.0; }
+        if (c == kGreedy) { k = 1; p = 1.0f; mp = 0.0f; }
         float uf = g.u ? g.u[row] : u01(rng4(g.state[0], g.state[1], kStream, (uint64_t)(g.row0 + row)).x);
         u = uf > 0.0f ? (uf < 0.99999994f ? (double)uf : 0.99999994039535522) : 0.0;
     }
@@ -70,12 +70,12 @@ MDP_DEV void wave_sync() {
 template <typename T, int G, int K>
 struct ShortRow {
     static constexpr int N = Chunk<T>::N, size = G, capacity = G;
-    static constexpr int per_lane = G < 8 ? 16 : G < 32 ? 8 : G <= 64 ? 4 : 256 / G;      // at most 256 buckets: their numbers are bytes
+    static constexpr int per_lane = G < 8 ? 16 : G <= 32 ? 8 : G <= 64 ? 4 : 256 / G;      // at most 256 buckets: their numbers are bytes
     static constexpr int W = G / 64;                   // waves of a block that holds one row
     static constexpr float window = 14.0f;
     static constexpr bool total_known = true;
     struct Listed { uint64_t word; double value; };      // the word rises in the order
-    struct Shared { Listed list[G]; double d[W ? W : 1]; uint32_t u[W ? W : 1]; uint32_t hist[per_lane * G]; int n; };
+    struct Shared { Listed list[G]; double d[W ? W : 1]; uint32_t u[W ? W : 1]; uint32_t hist[per_lane * G]; int n; float top; };
     float x[K][N];
     double w[K][N];
     int rank, shift;                                   // this lane's number; the row's shift
@@ -269,6 +269,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256, 4) void k_sample_short(SampleArgs
     q.hist = q.sh->hist;
     q.s = &s;
     m = q.highest(m);
+    if (lane == 0) q.sh->top = m;                      // for the end, where no register holds it: the same wave reads it, or behind barriers
     broken = q.some(broken) || s.c != s.c;
     const bool empty = m == -kInf;
 #pragma unroll
@@ -359,12 +360,9 @@ __global__ __launch_bounds__(G > 64 ? G : 256, 4) void k_sample_short(SampleArgs
     }
     g.actions[mine] = q.good ? found : -1;
     g.log_prob[mine] = q.good ? (float)log(found_w / mass) : broken ? __builtin_nanf("") : 0.0f;
-    if (__builtin_expect(q.good && found_w < kLight, 0)) {      // all that it takes is read again, and kept in no register until here
+    if (__builtin_expect(q.good && found_w < kLight, 0)) {      // what it takes is read again, and kept in no register until here
         const Row<T> again(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, mine);
-        float top = -kInf;
-#pragma unroll 1
-        for (int i = 0; i < again.V; ++i) top = larger(again.entry(i), top);
-        g.log_prob[mine] = log_share_of_light(again.entry(found), top, Settings(g, mine).c, mass);
+        g.log_prob[mine] = log_share_of_light(to_f32(again.x[found]), q.sh->top, Settings(g, mine).c, mass);
     }
 }
 
@@ -563,7 +561,7 @@ struct LongRow {
             }
             if (s.k == 0 && s.mp > 0.0) {
                 // lighter than min_p: never kept
-                const float light = (float)((double)m + log2(s.mp) / s.c);
+                const float light = (float)((double)m + log2((double)s.mp) / s.c);
                 bound = larger(light - 1e-3f * fabsf(light) - 1e-3f, bound);
             }
             if (lane == 0) sh.bound = bound;

@@ -62,11 +62,11 @@ MDP_DEV void wave_sync() {
 // Rows of up to G K chunks, 16 entries a lane: G lanes of a wave, or a block of G = 128 or 256, hold a row and its weights in
 // registers.  Groups of a wave go through their loops together until the last is done.
 //
-// Bound by instructions: 49152 x 256 float32 with top_p takes 46 us, 1700 vector instructions for a wave's four rows (300 of them the
+// Bound by instructions: 49152 x 256 float32 with top_p takes 43 us, 1665 vector instructions for a wave's four rows (300 of them the
 // weights), where the 50 MB are 11 us at the copy rate; uncut it takes 22.  Searching the border by halving the value range, sixteen
 // compares and 64-bit adds a step, took 71 where this took 44.  Entries and weights leave four waves a SIMD, and their 128 registers
-// do not hold all: 11 to 42 are spilled (2 or 3 where 256 lanes hold 16-bit rows), most of them by rows of up to 64 entries.  With five
-// waves (96 registers) what spills costs more: 53.
+// do not always hold all: up to 34 are spilled, most by rows of up to 64 entries, none by rows of one wave each.  With five waves (96
+// registers) what spills costs more: 53.
 template <typename T, int G, int K>
 struct ShortRow {
     static constexpr int N = Chunk<T>::N, size = G, capacity = G;
@@ -375,10 +375,10 @@ __global__ __launch_bounds__(G > 64 ? G : 256, 4) void k_sample_short(SampleArgs
 // listed and sorted, and everything exact happens on them.  Where no such value exists or too many entries lie above it (flat rows),
 // the border is searched over the whole row.
 //
-// 1024 x 131072 bfloat16 with top_p and min_p: 142 us for 268 MB (57 at the copy rate).  A row fills the registers of a CU, so while
+// 1024 x 131072 bfloat16 with top_p and min_p: 140 us for 268 MB (57 at the copy rate).  A row fills the registers of a CU, so while
 // it arrives (13 us of its share of the memory rate) nothing is left to do but its maxima and 32-bit mass, and the 15 us after it --
 // bound, list, sort -- load nothing.  Uncut rows of that size: 160 us, 64-bit weights of every entry; rows that the list leaves:
-// 641 us (scale 0.5), one pass for the list and four over the row, most of it from the caches.
+// 642 us (scale 0.5), one pass for the list and four over the row, most of it from the caches.
 template <typename T, bool MASK, int THREADS, int H>
 struct LongRow {
     static constexpr int N = Chunk<T>::N, W = THREADS / 64, size = THREADS, capacity = THREADS;
@@ -946,8 +946,8 @@ void launch_sample(const SampleArgs& g, hipStream_t s) {
     }
     SHORT(4) SHORT(8) SHORT(16) SHORT(32) SHORT(64)
     // From here to 4096 entries a row fits the registers of a block just as well; only a small top_k is quicker by the list of
-    // candidates (float32, 2^26 entries in rows of 1028 / 2048 / 4096: top_p 411 / 223 / 233 us against 1130 / 590 / 433 by list and
-    // whole row, top_k 40 388 / 199 / 207 against 272 / 144 / 90).
+    // candidates (float32, 2^26 entries in rows of 1028 / 2048 / 4096: top_p 412 / 220 / 240 us against 1130 / 590 / 433 by list and
+    // whole row, top_k 40 385 / 197 / 209 against 273 / 144 / 90).
     const bool few = !g.top_k && g.top_k_s > 0 && g.top_k_s <= 64;
     if (!few) { SHORT(128) SHORT(256) }
 #undef SHORT
@@ -961,7 +961,7 @@ void launch_sample(const SampleArgs& g, hipStream_t s) {
         hipLaunchKernelGGL((k_sample_whole<T, MASK, THREADS, 0, true>), grid, dim3(THREADS), 0, s, g);                          \
     }
     // Four blocks of 256 threads on a CU work on four rows in turn, one of 1024 on one: with many rows the former hide each other's
-    // waits (bfloat16 rows of 32000, top_p: 1024 of them 164 us against 216), with fewer than two a CU the latter is done sooner (256
+    // waits (bfloat16 rows of 32000, top_p: 1024 of them 162 us against 216), with fewer than two a CU the latter is done sooner (256
     // of them 55 us against 83).
     if (chunks <= 256 * 4) { LONG(256, 4) }
     else if (chunks <= 256 * 16 && g.rows >= 512) { LONG(256, 16) }

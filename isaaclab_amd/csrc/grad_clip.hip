@@ -5,9 +5,9 @@
 // Sums are held in 64 bits (the square of a float is exact there, so neither large nor small gradients leave the range) and
 // taken in an order that depends on the sizes and element types alone, not on where a tensor starts.
 //
-// Bound by memory: 160 M elements, half float32 and half bfloat16, into float32: 134 us for the 480 MB that the norm reads and 198 us
-// for the 1120 MB that the scaling reads and writes (part of them still cached), 330 us where three passes at the copy rate,
-// 4.7 TB/s, are 341; 50 M bfloat16 elements at an odd offset into float32 175.  An actor-critic of 0.57 M elements: 4.6 + 4.3 us, what
+// Bound by memory: 160 M elements, half float32 and half bfloat16, into float32: 133 us for the 480 MB that the norm reads and 197 us
+// for the 1120 MB that the scaling reads and writes (part of them still cached), 329 us where three passes at the copy rate,
+// 4.7 TB/s, are 341; 50 M bfloat16 elements at an odd offset into float32 175.  An actor-critic of 0.57 M elements: 4.4 + 3.9 us, what
 // two small launches take.  2048 partial sums instead of 1024 gain 2 % there and cost every block of the second launch a second
 // kilobyte-long read; stores past the caches lose 7 %.
 #include "mdp_device.hpp"

@@ -45,12 +45,15 @@ MDP_DEV float inverse_temperature(const float* per_row, float scalar, int64_t ro
     return t >= 1.17549435e-38f && t < kInf ? 1.0f / t : __builtin_nanf("");     // of a denormal it may be infinite
 }
 
+// Half of x - m, from hm = m / 2: stays in range whatever the signs, and is exact to the same bits; its factors are doubled.
+MDP_DEV float half_apart(float x, float hm) { return fmaf(x, 0.5f, -hm); }
+
 struct Running {
     float m;
     double s, t;                                       // of chunks that were summed up in 32 bits
     MDP_DEV static Running none() { return Running{-__FLT_MAX__, 0.0, 0.0}; }
     MDP_DEV void move(float to, float c) {             // about another maximum >= m
-        float d = (m - to) * c;
+        float d = half_apart(m, 0.5f * to) * c;
         d = d < -300.0f ? -300.0f : d;                 // 2^-300 is 0: 0 * inf must not arise
         const double f = (double)__builtin_amdgcn_exp2f(d);
         t = f * (t + (double)d * s);
@@ -60,10 +63,11 @@ struct Running {
     // n entries, none above m; summed on their own first: short chains of additions
     template <int N>
     MDP_DEV void add(const float (&v)[N], float c) {
+        const float hm = 0.5f * m;
         float cs = 0.0f, ct = 0.0f;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const float d = (v[e] - m) * c, w = __builtin_amdgcn_exp2f(d);
+            const float d = half_apart(v[e], hm) * c, w = __builtin_amdgcn_exp2f(d);
             cs += w;
             ct = fmaf(w, larger(d, -300.0f), ct);      // w is 0 there, and a NaN shows in s
         }
@@ -82,7 +86,7 @@ MDP_DEV void finish_row(const EvalArgs& g, const Row<T>& r, int64_t row, float m
     else if (a < 0 || a >= r.V) lp = __builtin_nanf("");
     else {
         const float x = r.entry((int)a);               // -inf: masked, or not allowed by itself, also where nothing is (ln s = -inf)
-        lp = x > -kInf || s != s ? (x - m) * inv_t - log_s : -kInf;
+        lp = x > -kInf || s != s ? half_apart(x, 0.5f * m) * (2.0f * inv_t) - log_s : -kInf;
     }
     g.log_prob[row] = lp;
     g.entropy[row] = h;
@@ -101,7 +105,7 @@ __global__ __launch_bounds__(256) void k_evaluate_short(EvalArgs g) {
     const int lane = threadIdx.x % G;
     if (row >= g.rows) return;
     const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
-    const float inv_t = inverse_temperature(g.temperature, g.temperature_s, row), c = inv_t * kLog2E;
+    const float inv_t = inverse_temperature(g.temperature, g.temperature_s, row), c = 2.0f * inv_t * kLog2E;
     float v[K][N];
 #pragma unroll
     for (int k = 0; k < K; ++k) r.template load<MASK>(k * G + lane, v[k]);
@@ -127,7 +131,7 @@ __global__ __launch_bounds__(256) void k_evaluate_long(EvalArgs g) {
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x;
     const Row<T> r(g.logits, g.ld, g.mask, g.ld_mask, g.vocab, row);
-    const float inv_t = inverse_temperature(g.temperature, g.temperature_s, row), c = inv_t * kLog2E;
+    const float inv_t = inverse_temperature(g.temperature, g.temperature_s, row), c = 2.0f * inv_t * kLog2E;
     const int first = r.full_first(), end = r.full_end();
     Running q = Running::none();
     for (int j0 = first + tid; j0 < end; j0 += 256 * B) {
@@ -181,13 +185,13 @@ __global__ __launch_bounds__(256) void k_evaluate_long(EvalArgs g) {
 // divided by T last.
 template <typename T>
 struct RowGrad {
-    float m, c, log2_s, a0, a1, hot, last;              // the last: 1 / T in a row whose other terms are not divided by T
+    float hm, c, log2_s, a0, a1, hot, last;             // the last: 1 / T in a row whose other terms are not divided by T
     int action;                                        // -1: none in the row
     bool whole;
     MDP_DEV RowGrad(const GradArgs& g, int64_t row) {
         const float inv_t = inverse_temperature(g.temperature, g.temperature_s, row);
-        m = g.stats[3 * row];
-        c = inv_t * kLog2E;
+        hm = 0.5f * g.stats[3 * row];
+        c = 2.0f * inv_t * kLog2E;
         const float log_s = g.stats[3 * row + 1], h = g.stats[3 * row + 2];
         log2_s = log_s == -kInf ? 0.0f : log_s * kLog2E;               // a row without allowed entries: p = 0 everywhere
         const int64_t a = g.actions[row];
@@ -210,12 +214,12 @@ struct RowGrad {
         }
     }
     MDP_DEV float operator()(float x) const {
-        const float lp = larger(fmaf(x - m, c, -log2_s), -300.0f);
+        const float lp = larger(fmaf(half_apart(x, hm), c, -log2_s), -300.0f);
         return __builtin_amdgcn_exp2f(lp) * fmaf(a1, lp, a0);
     }
     MDP_DEV float by_itself(float x, float own) const {
         if (x == -kInf) return 0.0f;
-        float lp = fmaf(x - m, c, -log2_s);
+        float lp = fmaf(half_apart(x, hm), c, -log2_s);
         lp = lp < -300.0f ? -300.0f : lp;              // a NaN stays
         return (__builtin_amdgcn_exp2f(lp) * fmaf(a1, lp, a0) + own) * last;
     }

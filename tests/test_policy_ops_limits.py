@@ -70,7 +70,9 @@ def roundings(x, a, lp, h, grad, gl, ge, mask, t, moves):
       log_prob   3 |d_a|, ln s, 1 of itself
       gradient   p: its exponent 4 |d|, log2 s as ln s and 2 more of itself, 1 of ln p, 2 for 2^x;  gl + ge (ln p + H): ge times what
                  ln p and H are off, 4 of each term;  1 / T: 1;  gl / T at the action: 2;  the result's own rounding
-    and a tenth more for products of these.  A p below 2^-126 is 0 in 32 bits: what it would give, its terms over T, is lost."""
+    and a tenth more for products of these.  Above T = 8.5e37, 1 / T is a denormal: T 2^-126 more wherever it enters (half a step,
+    2^-150, of 1 / T, in units of U), and half a step of what is made of it: gl + ge H and ge |log2 p| over T, their sum, gl / T, the
+    sum of that and the action's own.  A p below 2^-126 is 0 in 32 bits: what it would give, its terms over T, is lost."""
     ok = np.ones(len(x), bool) if mask is None else mask
     want = O.evaluate_row(x, a, mask, t, gl, ge)
     d = np.where(ok, (x[ok].max() - np.where(ok, x, 0.0)) / t, 0.0)
@@ -79,16 +81,19 @@ def roundings(x, a, lp, h, grad, gl, ge, mask, t, moves):
     p, ln_s = w / s, math.log(s)
     ln_p = np.where(ok, -d - ln_s, 0.0)
     mean, square = (p * d).sum(), (p * d * d).sum()
-    off_s = 5 * mean + 10 + 2 * moves
+    more = t * 2.0 ** -126
+    off_s = (5 + more) * mean + 10 + 2 * moves
     off_ln = off_s + 4 * ln_s
-    off_h = off_ln + 5 * square + (17 + 2 * moves) * mean + mean * off_s + abs(want[1])
+    off_h = off_ln + (5 + more) * square + (17 + more + 2 * moves) * mean + mean * off_s + abs(want[1])
     u = 1.1 * U
-    assert abs(lp - want[0]) <= u * (3 * d[a] + off_ln + abs(want[0])) + 1e-30, (lp, want[0])
+    assert abs(lp - want[0]) <= u * ((3 + more) * d[a] + off_ln + abs(want[0])) + 1e-30, (lp, want[0])
     assert abs(h - want[1]) <= u * off_h + 1e-30, (h, want[1])
-    off_lnp = 4 * d + off_ln + 2 * ln_s + np.abs(ln_p)
+    off_lnp = (4 + more) * d + off_ln + 2 * ln_s + np.abs(ln_p)
     terms = abs(gl) + abs(ge) * (np.abs(ln_p) + abs(want[1]))
-    tol = p * ((off_lnp + 2) * np.abs(gl + ge * (ln_p + want[1])) + abs(ge) * (off_lnp + off_h) + 5 * terms) * u / t
-    tol[a] += 2 * u * abs(gl) / t
+    tol = p * ((off_lnp + 2) * np.abs(gl + ge * (ln_p + want[1])) + abs(ge) * (off_lnp + off_h) + (5 + more) * terms) * u / t
+    tol[a] += (2 + more) * u * abs(gl) / t
+    tol += 2.0 ** -150 * p * (2 + np.abs(ln_p) / math.log(2))
+    tol[a] += 2.0 ** -149
     tol += 2.0 ** -126 * terms / t
     return want, tol
 
@@ -369,3 +374,26 @@ def test_seeding_behind_a_capture(device, seed):
     reseed(8)
     assert torch.equal(rl.sample_categorical(x)[0], inside)
     M.seed_samplers(1, device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [9, 700, 3000, 9001, 40000])
+def test_logits_further_apart_than_the_largest_number(device, dtype, vocab):
+    """Logits of both signs near the ends of the range, at temperatures that bring them together again: their differences are beyond
+    32 bits, what is drawn and evaluated is not."""
+    g = rng_of("ends", dtype, vocab)
+    top = torch.finfo(DT[dtype]).max
+    x = ((torch.rand(6, vocab, generator=g) * 2 - 1) * top).to(DT[dtype])
+    x[:, 0], x[:, 1] = -top, top
+    a = torch.randint(0, vocab, (6,), generator=g)
+    a[0], a[1] = 0, 1
+    u = torch.rand(6, generator=g)
+    gl, ge = (torch.randn(6, generator=g) for _ in range(2))
+    x, a, u, gl, ge = (v.to(device) for v in (x, a, u, gl, ge))
+    moves = 0 if vocab < 2000 else vocab // 4096 + 3
+    for t in (3e38, 1e38, 1e37):
+        for s in (dict(), dict(top_p=0.9), dict(top_k=vocab // 2), dict(min_p=0.1)):
+            check_draw(x, u, rl.sample_categorical(x, u, temperature=t, **s), temperature=t, **s)
+        check_roundings(x, a, *run_evaluation(x, a, gl, ge, temperature=t), gl, ge, temperature=t, moves=moves)
+    assert rl.evaluate_categorical(x, a, temperature=1.0)[0][0].item() == -math.inf
